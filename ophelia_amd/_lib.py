@@ -122,8 +122,44 @@ VOCODER_SIGNATURES = {
     "oph_vocoder_last_device_ms": (C.c_int, [C.c_void_p, c_f32p]),
 }
 
+
+class OphSeqAttn(C.Structure):
+    _fields_ = ([(n, C.c_void_p) for n in ("q", "k", "v", "out", "lse", "dout", "dq", "dk", "dv", "q_lens", "k_lens", "mask")] +
+                [(n, C.c_int64 * 3) for n in ("q_stride", "k_stride", "v_stride", "dout_stride")] + [("mask_stride", C.c_int64 * 2)] +
+                [("workspace", C.c_void_p), ("workspace_bytes", C.c_size_t)] +
+                [(n, C.c_int32) for n in ("B", "Tq", "Tk", "Hq", "Hk", "D", "dtype")] + [("scale", C.c_float)])
+
+
+class OphSeqRecur(C.Structure):
+    _fields_ = ([(n, C.c_void_p) for n in ("x", "gate", "h0", "h", "h_last", "dh", "dh_last", "dx", "dgate", "dh0", "lens")] +
+                [(n, C.c_int64 * 2) for n in ("x_stride", "gate_stride", "h_stride", "dh_stride")] +
+                [("workspace", C.c_void_p), ("workspace_bytes", C.c_size_t)] + [(n, C.c_int32) for n in ("B", "T", "C", "dtype")])
+
+
+SEQ_F32, SEQ_BF16, SEQ_F16 = 0, 1, 2
+# every symbol declared in include/ophelia_seq.h
+SEQ_LIBPATH = os.path.join(LIBDIR, "libophelia_seq.so")
+SEQ_SOURCES = ["oph_seq.hip", "oph_attn.hip", "oph_attngrad.hip", "oph_embed.hip", "oph_recur.hip"]
+SEQ_HEADERS = ["oph_seq.h", "oph_attn.h"]
+SEQ_SIGNATURES = {
+    "oph_seq_abi_version": (C.c_int, []),
+    "oph_seq_last_error": (C.c_char_p, []),
+    "oph_seq_attn_workspace": (C.c_int64, [C.POINTER(OphSeqAttn), C.c_int]),
+    "oph_seq_attn_forward": (C.c_int, [C.POINTER(OphSeqAttn), C.c_int, C.c_void_p]),
+    "oph_seq_attn_gradient": (C.c_int, [C.POINTER(OphSeqAttn), C.c_int, C.c_void_p]),
+    "oph_seq_embed_lookup": (C.c_int, [C.c_void_p, C.c_int, C.c_int64, C.c_void_p, C.c_int64, C.c_int, C.c_int, C.c_float, C.c_int, C.c_int,
+                                       C.c_void_p, C.c_int, C.c_void_p]),
+    "oph_seq_embed_workspace": (C.c_int64, [C.c_int64, C.c_int, C.c_int]),
+    "oph_seq_embed_gradient": (C.c_int, [C.c_void_p, C.c_int, C.c_int64, C.c_void_p, C.c_int64, C.c_int, C.c_int, C.c_float, C.c_int, C.c_int,
+                                         C.c_void_p, C.c_void_p, C.c_size_t, C.c_int, C.c_void_p]),
+    "oph_seq_recur_workspace": (C.c_int64, [C.POINTER(OphSeqRecur), C.c_int]),
+    "oph_seq_recur_forward": (C.c_int, [C.POINTER(OphSeqRecur), C.c_int, C.c_void_p]),
+    "oph_seq_recur_gradient": (C.c_int, [C.POINTER(OphSeqRecur), C.c_int, C.c_void_p]),
+}
+
 _lib = None
 _vlib = None
+_slib = None
 
 
 class OpheliaHipError(RuntimeError):
@@ -175,6 +211,10 @@ def build(verbose=False):
     vsrcs = [os.path.join(CSRC, s) for s in VOCODER_SOURCES]
     _hipcc_shared(VOCODER_LIBPATH, vsrcs, vsrcs + [os.path.join(inc, "ophelia_vocoder.h")],
                   ["-L/opt/rocm/lib", "-lhipfft", "-Wl,-rpath,/opt/rocm/lib"], verbose)
+    # packed fp32 instructions stay off: some of their forms have given wrong results on this hardware
+    ssrcs = [os.path.join(CSRC, s) for s in SEQ_SOURCES]
+    _hipcc_shared(SEQ_LIBPATH, ssrcs, ssrcs + [os.path.join(CSRC, h) for h in SEQ_HEADERS] + [os.path.join(inc, "ophelia_seq.h"), os.path.join(inc, "ophelia_hip.h")],
+                  ["-fvisibility=hidden", "-Xclang", "-target-feature", "-Xclang", "-packed-fp32-ops"], verbose)
     return libpath()
 
 
@@ -216,6 +256,26 @@ def load_vocoder():
     if lib.oph_vocoder_abi_version() != 1:
         raise OpheliaHipError("vocoder ABI version mismatch")
     _vlib = lib
+    return lib
+
+
+def load_seq():
+    """Load libophelia_seq.so (operators on device tensors).  Raises if it is not built."""
+    global _slib
+    if _slib is not None:
+        return _slib
+    if not os.path.exists(SEQ_LIBPATH):
+        raise OpheliaHipError(
+            "HIP extension %s is missing: run `python -c 'import __graft_entry__ as g; g.build()'` "
+            "(there is no CPU fallback)" % SEQ_LIBPATH)
+    lib = C.CDLL(SEQ_LIBPATH)
+    for name, (res, args) in SEQ_SIGNATURES.items():
+        fn = getattr(lib, name)
+        fn.restype = res
+        fn.argtypes = args
+    if lib.oph_seq_abi_version() != 1:
+        raise OpheliaHipError("sequence-operator ABI version mismatch")
+    _slib = lib
     return lib
 
 

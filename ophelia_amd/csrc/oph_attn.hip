@@ -1,0 +1,388 @@
+// Cross attention, forward: oph_seq_attn_forward.
+#include "oph_attn.h"
+#include "../../include/ophelia_hip.h"
+
+#include <math.h>
+
+namespace ophseq {
+
+// Running softmax of one query column: m in units of log2, l the sum over this lane's half of the keys.
+struct Soft { float m, l; };
+
+// Scores of KT keys x 32 queries (rows x columns) -> probabilities in place; returns the factor by which earlier results shrink.
+template <int N> __device__ __forceinline__ float soft_step(f32x16 (&S)[N], uint64_t bits, Soft& st, float c, int half) {
+    constexpr uint64_t FULL = N == 2 ? ~0ull : 0xffffffffull;
+    if (bits != FULL) {
+#pragma unroll
+        for (int n = 0; n < N; ++n) {
+            const uint32_t b = (uint32_t)(bits >> (32 * n)) >> (4 * half);
+#pragma unroll
+            for (int r = 0; r < 16; ++r) S[n][r] = (b >> (8 * (r / 4) + r % 4)) & 1 ? S[n][r] : -INFINITY;
+        }
+    }
+    float mx = -INFINITY;
+#pragma unroll
+    for (int n = 0; n < N; ++n)
+#pragma unroll
+        for (int r = 0; r < 16; ++r) mx = fmaxf(mx, S[n][r]);
+    mx = fmaxf(mx, other_half(mx));
+    const float m = fmaxf(st.m, mx * c);
+    const float base = m == -INFINITY ? 0.f : m;       // a row without a finite score so far: every exponential below is 0
+    const float shrink = exp2_(st.m - base);
+    float sum = 0.f;
+#pragma unroll
+    for (int n = 0; n < N; ++n)
+#pragma unroll
+        for (int r = 0; r < 16; ++r) {
+            S[n][r] = exp2_(fmaf(S[n][r], c, -base));
+            sum += S[n][r];
+        }
+    st.l = st.l * shrink + sum;
+    st.m = m;
+    return shrink;
+}
+
+// ---- many rows: a workgroup of 4 waves, 32*NQ rows each, over all keys; key and value tiles in LDS for the four -----------------------
+template <class T, int DP, int KT, int NQ>
+__global__ __launch_bounds__(256) void attn_wide(const AttnP p) {
+    constexpr int ROWS = 128 * NQ, NK = KT / 32, TB = Tile<T, DP>::bytes(KT);
+    __shared__ __attribute__((aligned(16))) char lds[4 * TB];
+    const int tid = threadIdx.x, lane = tid & 63, wave = tid >> 6, half = lane >> 5, col = lane & 31;
+    const int M = p.Tq * p.G, tiles = (M + ROWS - 1) / ROWS;
+    const Where w = where(p, on_xcd(blockIdx.x, tiles * p.B * p.Hk), tiles);
+    const int row0 = w.tile * ROWS + wave * 32 * NQ;
+    const float c = p.scale * LOG2E;
+
+    frag_t<T> Q[NQ][DP / 16];
+    f32x16 O[NQ][DP / 32];
+    Soft st[NQ];
+#pragma unroll
+    for (int n = 0; n < NQ; ++n) {
+        const int r = row0 + n * 32 + col;
+        row_frags<T, DP>(Q[n], row_ptr<T>(p, p.q, w, r, p.qs[0], p.qs[1], p.qs[2]), p.D, r < M && row_time(p, r) < w.qlen, half);
+        st[n] = Soft{-INFINITY, 0.f};
+#pragma unroll
+        for (int d = 0; d < DP / 32; ++d) O[n][d] = f32x16{};
+    }
+
+    const T* k = (const T*)p.k + w.b * p.ks[0] + w.hk * p.ks[2];
+    const T* v = (const T*)p.v + w.b * p.vs[0] + w.hk * p.vs[2];
+    const bool any = row_time(p, w.tile * ROWS) < w.qlen;               // a tile of padding only: nothing to read
+    const int nt = any ? (w.klen + KT - 1) / KT : 0;
+    Stage<T, DP, KT, 256> sk, sv;
+    uint64_t bits = 0, next = 0;
+    auto fetch = [&](int j) {
+        const int key0 = j * KT, last = w.klen - 1;
+        next = key_bits(p, w, key0, w.klen, lane) & (KT == 64 ? ~0ull : 0xffffffffull);
+        sk.load([&](int r) { return k + (int64_t)min(key0 + r, last) * p.ks[1]; }, p.D, tid);
+        sv.load([&](int r) { return v + (int64_t)min(key0 + r, last) * p.vs[1]; }, p.D, tid);
+    };
+    auto commit = [&](int j) {
+        char* t = lds + (j & 1) * 2 * TB;
+        sk.store(t, next, p.D, tid);
+        sv.store(t + TB, next, p.D, tid);
+        bits = next;
+    };
+    if (nt) { fetch(0); commit(0); }
+    for (int j = 0; j < nt; ++j) {
+        const uint64_t now = bits;
+        __syncthreads();
+        if (j + 1 < nt) fetch(j + 1);
+        if (now) {
+            const char* tk = lds + (j & 1) * 2 * TB;
+            f32x16 S[NQ][NK];
+#pragma unroll
+            for (int n = 0; n < NQ; ++n)
+#pragma unroll
+                for (int i = 0; i < NK; ++i) S[n][i] = f32x16{};
+#pragma unroll
+            for (int s = 0; s < DP / 16; ++s)
+#pragma unroll
+                for (int i = 0; i < NK; ++i) {
+                    const frag_t<T> a = row_frag<T, DP>(tk, 32 * i, s, lane);
+#pragma unroll
+                    for (int n = 0; n < NQ; ++n) S[n][i] = El<T>::mma(a, Q[n][s], S[n][i]);
+                }
+#pragma unroll
+            for (int n = 0; n < NQ; ++n) {
+                const float shrink = soft_step<NK>(S[n], now, st[n], c, half);
+                if (__any(shrink != 1.f)) {
+#pragma unroll
+                    for (int d = 0; d < DP / 32; ++d) O[n][d] *= shrink;
+                }
+            }
+            const char* tv = tk + TB;
+#pragma unroll
+            for (int i = 0; i < NK; ++i)
+#pragma unroll
+                for (int s = 0; s < 2; ++s) {
+                    frag_t<T> P[NQ];
+#pragma unroll
+                    for (int n = 0; n < NQ; ++n) P[n] = next_frag<T>(S[n][i], s);
+#pragma unroll
+                    for (int d = 0; d < DP / 32; ++d) {
+                        const frag_t<T> a = trans_frag<T, DP>(tv, 32 * i + 16 * s, 32 * d, lane);
+#pragma unroll
+                        for (int n = 0; n < NQ; ++n) O[n][d] = El<T>::mma(a, P[n], O[n][d]);
+                    }
+                }
+        }
+        if (j + 1 < nt) commit(j + 1);
+    }
+
+#pragma unroll
+    for (int n = 0; n < NQ; ++n) {
+        const int r = row0 + n * 32 + col;
+        const float l = st[n].l + other_half(st[n].l);
+        const int t = row_time(p, r), h = w.hk * p.G + r - t * p.G;
+        if (r < M) {
+            const bool live = t < w.qlen && l != 0.f;                  // NaN stays NaN
+            const float inv = live ? 1.f / l : 0.f;
+            T* o = (T*)p.o0 + (((int64_t)w.b * p.Tq + t) * (p.Hk * p.G) + h) * p.D;
+#pragma unroll
+            for (int d = 0; d < DP / 32; ++d)
+#pragma unroll
+                for (int g = 0; g < 4; ++g) {
+                    const int at = 32 * d + 8 * g + 4 * half;
+                    const f32x4 x = {O[n][d][4 * g], O[n][d][4 * g + 1], O[n][d][4 * g + 2], O[n][d][4 * g + 3]};
+                    if (at < p.D) store4<T>(o + at, live ? x * inv : f32x4{0.f, 0.f, 0.f, 0.f});
+                }
+            if (half == 0) p.lse[((int64_t)w.b * (p.Hk * p.G) + h) * p.Tq + t] = live ? (st[n].m + log2f(l)) * LN2 : -INFINITY;
+        }
+    }
+}
+
+// ---- few rows: a workgroup of 4 waves shares 32 rows, every wave takes every fourth tile of 32 keys of its split; keys go straight
+// to the matrix operand, values through a tile of the wave's own.  With nsplit > 1 the results of the splits meet in attn_join. ----
+template <class T, int DP>
+__global__ __launch_bounds__(256) void attn_split(const AttnP p) {
+    constexpr int TB = Tile<T, DP>::bytes(32);
+    constexpr int JOIN = 4 * 32 * 36 * 4;
+    __shared__ __attribute__((aligned(16))) char lds[4 * TB > JOIN ? 4 * TB : JOIN];
+    __shared__ float ml[4][32][2];
+    const int tid = threadIdx.x, lane = tid & 63, wave = tid >> 6, half = lane >> 5, col = lane & 31;
+    const int M = p.Tq * p.G, tiles = (M + 31) / 32;
+    const int lin = on_xcd(blockIdx.x, tiles * p.B * p.Hk * p.nsplit), split = lin % p.nsplit;
+    const Where w = where(p, lin / p.nsplit, tiles);
+    const int row0 = w.tile * 32;
+    const float c = p.scale * LOG2E;
+    const int per = ((w.klen + 31) / 32 + p.nsplit - 1) / p.nsplit * 32;
+    const int kbeg = split * per, kend = row_time(p, row0) < w.qlen ? min(w.klen, kbeg + per) : kbeg;
+
+    frag_t<T> Q[DP / 16];
+    f32x16 O[DP / 32];
+    Soft st = {-INFINITY, 0.f};
+    {
+        const int r = row0 + col;
+        row_frags<T, DP>(Q, row_ptr<T>(p, p.q, w, r, p.qs[0], p.qs[1], p.qs[2]), p.D, r < M && row_time(p, r) < w.qlen, half);
+    }
+#pragma unroll
+    for (int d = 0; d < DP / 32; ++d) O[d] = f32x16{};
+    const T* k = (const T*)p.k + w.b * p.ks[0] + w.hk * p.ks[2];
+    const T* v = (const T*)p.v + w.b * p.vs[0] + w.hk * p.vs[2];
+    char* tv = lds + wave * TB;
+    for (int key0 = kbeg + wave * 32; key0 < kend; key0 += 128) {
+        const uint64_t bits = key_bits(p, w, key0, kend, lane) & 0xffffffffull;
+        if (!bits) continue;
+        Stage<T, DP, 32, 64> sv;
+        frag_t<T> K[DP / 16];
+        row_frags<T, DP>(K, k + (int64_t)min(key0 + col, kend - 1) * p.ks[1], p.D, true, half);
+        sv.load([&](int r) { return v + (int64_t)min(key0 + r, kend - 1) * p.vs[1]; }, p.D, lane);
+        f32x16 S[1] = {f32x16{}};
+#pragma unroll
+        for (int s = 0; s < DP / 16; ++s) S[0] = El<T>::mma(K[s], Q[s], S[0]);
+        const float shrink = soft_step<1>(S, bits, st, c, half);
+        if (__any(shrink != 1.f)) {
+#pragma unroll
+            for (int d = 0; d < DP / 32; ++d) O[d] *= shrink;
+        }
+        wave_lds_fence();
+        sv.store(tv, bits, p.D, lane);
+        wave_lds_fence();
+#pragma unroll
+        for (int s = 0; s < 2; ++s) {
+            const frag_t<T> P = next_frag<T>(S[0], s);
+#pragma unroll
+            for (int d = 0; d < DP / 32; ++d) O[d] = El<T>::mma(trans_frag<T, DP>(tv, 16 * s, 32 * d, lane), P, O[d]);
+        }
+    }
+
+    // the four waves' results: the common maximum, then 32 columns of D at a time through LDS, in the order of the waves
+    const float lw = st.l + other_half(st.l);
+    if (half == 0) { ml[wave][col][0] = st.m; ml[wave][col][1] = lw; }
+    __syncthreads();
+    float m = -INFINITY;
+#pragma unroll
+    for (int i = 0; i < 4; ++i) m = fmaxf(m, ml[i][col][0]);
+    const float weight = exp2_(st.m - (m == -INFINITY ? 0.f : m));
+    const int orow = tid >> 3, od = (tid & 7) * 4, r = row0 + orow;    // what this thread writes
+    float om = -INFINITY, l = 0.f;
+#pragma unroll
+    for (int i = 0; i < 4; ++i) om = fmaxf(om, ml[i][orow][0]);
+#pragma unroll
+    for (int i = 0; i < 4; ++i) l += ml[i][orow][1] * exp2_(ml[i][orow][0] - (om == -INFINITY ? 0.f : om));
+    const int t = row_time(p, r), h = w.hk * p.G + r - t * p.G;
+    const bool live = r < M && t < w.qlen && l != 0.f;
+    const float inv = live ? 1.f / l : 0.f;
+    const int64_t unit = ((int64_t)(w.b * p.Hk + w.hk) * tiles + w.tile) * p.nsplit + split;
+    float* x = (float*)lds;
+#pragma unroll
+    for (int d = 0; d < DP / 32; ++d) {
+        __syncthreads();
+#pragma unroll
+        for (int g = 0; g < 4; ++g) {
+            const f32x4 y = {O[d][4 * g], O[d][4 * g + 1], O[d][4 * g + 2], O[d][4 * g + 3]};
+            *(f32x4*)(x + (wave * 32 + col) * 36 + 8 * g + 4 * half) = y * weight;
+        }
+        __syncthreads();
+        f32x4 sum = *(const f32x4*)(x + orow * 36 + od);
+#pragma unroll
+        for (int i = 1; i < 4; ++i) sum += *(const f32x4*)(x + (i * 32 + orow) * 36 + od);
+        const int at = 32 * d + od;
+        if (r < M && at < p.D) {
+            if (p.nsplit == 1)
+                store4<T>((T*)p.o0 + (((int64_t)w.b * p.Tq + t) * (p.Hk * p.G) + h) * p.D + at, live ? sum * inv : f32x4{0.f, 0.f, 0.f, 0.f});
+            else
+                *(f32x4*)(p.part + (unit * 32 + orow) * DP + at) = sum;
+        }
+    }
+    if ((tid & 7) == 0 && r < M) {
+        if (p.nsplit == 1)
+            p.lse[((int64_t)w.b * (p.Hk * p.G) + h) * p.Tq + t] = live ? (om + log2f(l)) * LN2 : -INFINITY;
+        else {
+            p.aux[(unit * 32 + orow) * 2] = om;
+            p.aux[(unit * 32 + orow) * 2 + 1] = l;
+        }
+    }
+}
+
+// one wave per row: the splits' results, weighted to the common maximum, in the order of the splits (at most 64 of them)
+template <class T, int DP>
+__global__ __launch_bounds__(256) void attn_join(const AttnP p) {
+    const int lane = threadIdx.x & 63, M = p.Tq * p.G, tiles = (M + 31) / 32;
+    const int64_t row = (int64_t)blockIdx.x * 4 + (threadIdx.x >> 6);
+    if (row >= (int64_t)p.B * p.Hk * M) return;
+    const int bh = (int)(row / M), r = (int)(row - (int64_t)bh * M);
+    const int b = bh / p.Hk, hk = bh - b * p.Hk, t = row_time(p, r), h = hk * p.G + r - t * p.G;
+    const int qlen = p.q_lens ? clampi(p.q_lens[b], 0, p.Tq) : p.Tq;
+    const int64_t unit = ((int64_t)bh * tiles + r / 32) * p.nsplit;
+    float m = -INFINITY, l = 0.f;
+    if (lane < p.nsplit) {
+        const float* at = p.aux + ((unit + lane) * 32 + r % 32) * 2;
+        m = at[0];
+        l = at[1];
+    }
+    float all = m;
+#pragma unroll
+    for (int i = 32; i; i >>= 1) all = fmaxf(all, __shfl_xor(all, i));
+    const float weight = exp2_(m - (all == -INFINITY ? 0.f : all));
+    float sum = l * weight;
+#pragma unroll
+    for (int i = 32; i; i >>= 1) sum += __shfl_xor(sum, i);
+    const int d = lane * 4;
+    f32x4 o = {0.f, 0.f, 0.f, 0.f};
+    for (int s = 0; s < p.nsplit; ++s) {
+        const float ws = __shfl(weight, s);
+        if (d < p.D) o += *(const f32x4*)(p.part + ((unit + s) * 32 + r % 32) * DP + d) * ws;
+    }
+    const bool live = t < qlen && sum != 0.f;
+    const float inv = live ? 1.f / sum : 0.f;
+    if (d < p.D) store4<T>((T*)p.o0 + (((int64_t)b * p.Tq + t) * (p.Hk * p.G) + h) * p.D + d, live ? o * inv : f32x4{0.f, 0.f, 0.f, 0.f});
+    if (lane == 0) p.lse[((int64_t)b * (p.Hk * p.G) + h) * p.Tq + t] = live ? (all + log2f(sum)) * LN2 : -INFINITY;
+}
+
+// ---- host side --------------------------------------------------------------------------------------------------------------------
+int attn_check(const oph_seq_attn* a, bool gradient) {
+    if (!a) return fail(OPH_ERR_INVALID, "attention: no arguments");
+    if (!type_bytes(a->dtype)) return fail(OPH_ERR_INVALID, "attention: dtype %d is not one of OPH_SEQ_*", a->dtype);
+    if (a->B < 0 || a->Tq < 0 || a->Tk < 0) return fail(OPH_ERR_INVALID, "attention: negative size (B %d, Tq %d, Tk %d)", a->B, a->Tq, a->Tk);
+    if (a->Hq < 1 || a->Hk < 1 || a->Hq % a->Hk) return fail(OPH_ERR_INVALID, "attention: %d query heads are not a multiple of %d key heads", a->Hq, a->Hk);
+    if (a->D < 8 || a->D > 256 || a->D % 8) return fail(OPH_ERR_UNSUPPORTED, "attention: head size %d is not a multiple of 8 up to 256", a->D);
+    if (!(a->scale > 0.f) || !(a->scale < INFINITY)) return fail(OPH_ERR_INVALID, "attention: scale %g is not positive and finite", (double)a->scale);
+    // 32-bit row and workgroup numbers; the division by the group size is exact below the first bound
+    if ((double)a->Tq * a->Hq / a->Hk * (a->Hq / a->Hk) > 2147483647.0 || (double)a->B * a->Hq * ((double)a->Tq + a->Tk + 64) > 4.0e9 || a->Tk > 2147483000 - 256 ||
+        a->Tq > 2147483000 - 256 || (double)a->B * a->Hq > 1.0e7)
+        return fail(OPH_ERR_UNSUPPORTED, "attention: too many rows (B %d, Tq %d, Tk %d, Hq %d)", a->B, a->Tq, a->Tk, a->Hq);
+    (void)gradient;
+    return OPH_OK;
+}
+
+AttnP attn_params(const oph_seq_attn* a) {
+    AttnP p = {};
+    p.q = a->q; p.k = a->k; p.v = a->v;
+    p.q_lens = a->q_lens; p.k_lens = a->k_lens; p.mask = a->mask;
+    for (int i = 0; i < 3; ++i) { p.qs[i] = a->q_stride[i]; p.ks[i] = a->k_stride[i]; p.vs[i] = a->v_stride[i]; }
+    p.ms[0] = a->mask_stride[0]; p.ms[1] = a->mask_stride[1];
+    p.B = a->B; p.Tq = a->Tq; p.Tk = a->Tk; p.Hk = a->Hk; p.G = a->Hq / a->Hk; p.D = a->D;
+    p.magic = p.G > 1 ? (unsigned)(((1ull << 32) + p.G - 1) / p.G) : 0;
+    p.scale = a->scale;
+    p.nsplit = 1;
+    return p;
+}
+
+static int pad_d(int D) { return D <= 64 ? 64 : D <= 128 ? 128 : 256; }
+
+struct FwdPlan { bool wide; int nsplit; int64_t units; };
+static FwdPlan forward_plan(const oph_seq_attn* a) {
+    const int64_t M = (int64_t)a->Tq * (a->Hq / a->Hk), heads = (int64_t)a->B * a->Hk;
+    FwdPlan f;
+    f.wide = cdiv(M, 128) * heads >= 256;
+    f.units = cdiv(M, 32) * heads;
+    const int64_t fill = cdiv(512, f.units > 0 ? f.units : 1), most = cdiv(a->Tk, 128);
+    const int64_t n = fill < most ? fill : most;
+    f.nsplit = f.wide ? 1 : (int)(n < 1 ? 1 : n > 64 ? 64 : n);
+    return f;
+}
+
+int64_t attn_forward_workspace(const oph_seq_attn* a) {
+    const FwdPlan f = forward_plan(a);
+    return f.nsplit == 1 ? 0 : f.units * f.nsplit * 32 * (pad_d(a->D) + 2) * (int64_t)sizeof(float);
+}
+
+template <class T, int DP, int KT, int NQ> static int forward(const oph_seq_attn* a, const FwdPlan& f, AttnP& p, void* stream) {
+    const int64_t M = (int64_t)p.Tq * p.G, heads = (int64_t)p.B * p.Hk;
+    if (f.wide) return launch<AttnP>(attn_wide<T, DP, KT, NQ>, dim3((unsigned)(cdiv(M, 128 * NQ) * heads)), 256, p, 0, stream);
+    p.nsplit = f.nsplit;
+    p.part = (float*)a->workspace;
+    p.aux = p.part + f.units * f.nsplit * 32 * DP;
+    if (int rc = launch<AttnP>(attn_split<T, DP>, dim3((unsigned)(f.units * f.nsplit)), 256, p, 0, stream)) return rc;
+    if (f.nsplit > 1) return launch<AttnP>(attn_join<T, DP>, dim3((unsigned)cdiv(M * heads, 4)), 256, p, 0, stream);
+    return OPH_OK;
+}
+template <class T> static int forward_d(const oph_seq_attn* a, const FwdPlan& f, AttnP& p, void* stream) {
+    constexpr int KT = sizeof(T) == 2 ? 64 : 32;
+    if (p.D <= 64) return forward<T, 64, 64, 1>(a, f, p, stream);
+    if (p.D <= 128) return forward<T, 128, KT, 1>(a, f, p, stream);
+    return forward<T, 256, 32, 1>(a, f, p, stream);
+}
+
+}  // namespace ophseq
+
+using namespace ophseq;
+extern "C" {
+
+int64_t oph_seq_attn_workspace(const oph_seq_attn* a, int gradient) {
+    if (int rc = attn_check(a, gradient != 0)) return rc;
+    if (!a->B || !a->Tq) return gradient && a->B && a->Tk ? attn_gradient_workspace(a) : 0;
+    return gradient ? attn_gradient_workspace(a) : attn_forward_workspace(a);
+}
+
+int oph_seq_attn_forward(const oph_seq_attn* a, int device, void* stream) {
+    if (int rc = attn_check(a, false)) return rc;
+    if (!a->B || !a->Tq) return OPH_OK;
+    if (!a->q || !a->out || !a->lse || (a->Tk && (!a->k || !a->v))) return fail(OPH_ERR_INVALID, "attention: q, k, v, out and lse must not be NULL");
+    const int64_t need = attn_forward_workspace(a);
+    if (need && (!a->workspace || (int64_t)a->workspace_bytes < need || ((uintptr_t)a->workspace & 15)))
+        return fail(OPH_ERR_INVALID, "attention: the workspace must hold %lld bytes, 16-byte aligned", (long long)need);
+    OnDevice on(device);
+    if (on.status) return on.status;
+    const FwdPlan f = forward_plan(a);
+    AttnP p = attn_params(a);
+    p.o0 = a->out;
+    p.lse = a->lse;
+    if (a->dtype == OPH_SEQ_F32) return forward_d<float>(a, f, p, stream);
+    if (a->dtype == OPH_SEQ_BF16) return forward_d<bf16_t>(a, f, p, stream);
+    return forward_d<f16_t>(a, f, p, stream);
+}
+
+}  // extern "C"

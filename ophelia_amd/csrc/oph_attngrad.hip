@@ -1,0 +1,341 @@
+// Cross attention, gradient: oph_seq_attn_gradient.
+//
+// Two passes, each of which owns what it writes, so that no sum depends on an order of arrival: attn_dq (a workgroup owns 128 rows and
+// runs over the keys) also forms delta = dout.out for attn_dkv (a workgroup owns 128 keys and runs over the rows).  Both recompute the
+// scores from q, k and the forward's lse: 7 products of Tq x Tk x D instead of 5, for nothing to add up across workgroups.
+#include "oph_attn.h"
+#include "../../include/ophelia_hip.h"
+
+#include <math.h>
+
+namespace ophseq {
+
+__device__ __forceinline__ float dot8(f32x8 a, f32x8 b) {
+    float s = 0.f;
+#pragma unroll
+    for (int j = 0; j < 8; ++j) s = fmaf(a[j], b[j], s);
+    return s;
+}
+
+// ---- dq: S^T = K q^T and dP^T = V dout^T have the queries as columns; dS^T is the operand of dq^T = K^T dS^T -------------------------------
+template <class T, int DP>
+__global__ __launch_bounds__(256) void attn_dq(const AttnP p) {
+    constexpr int KT = 32, TB = Tile<T, DP>::bytes(KT);
+    __shared__ __attribute__((aligned(16))) char lds[4 * TB];
+    const int tid = threadIdx.x, lane = tid & 63, wave = tid >> 6, half = lane >> 5, col = lane & 31;
+    const int M = p.Tq * p.G, Hq = p.Hk * p.G, tiles = (M + 127) / 128;
+    const int lin = on_xcd(blockIdx.x, tiles * p.B * p.Hk * p.nsplit), split = lin % p.nsplit;
+    const Where w = where(p, lin / p.nsplit, tiles);
+    const int r = w.tile * 128 + wave * 32 + col, t = row_time(p, r), h = w.hk * p.G + r - t * p.G;
+    const bool row = r < M && t < w.qlen;
+    const float c = p.scale * LOG2E;
+
+    frag_t<T> Q[DP / 16], dO[DP / 16];
+    f32x16 dQ[DP / 32];
+    row_frags<T, DP>(Q, row_ptr<T>(p, p.q, w, r, p.qs[0], p.qs[1], p.qs[2]), p.D, row, half);
+    row_frags<T, DP>(dO, row_ptr<T>(p, p.dout, w, r, p.ds[0], p.ds[1], p.ds[2]), p.D, row, half);
+    float delta = 0.f, lse2 = INFINITY;                   // exp2(s - inf) = 0: rows that are not there or that saw no key
+    {
+        const T* o = row_ptr<T>(p, p.out, w, r, (int64_t)p.Tq * Hq * p.D, (int64_t)Hq * p.D, p.D);
+#pragma unroll
+        for (int s = 0; s < DP / 16; ++s) {
+            const int d = s * 16 + half * 8;
+            const T* at = o + (d < p.D ? d : 0);
+            const frag_t<T> x = bits_to_frag<T>(load16(at), sizeof(T) == 4 ? load16(at + 4) : u32x4{0, 0, 0, 0});
+            delta += dot8(__builtin_convertvector(x, f32x8), __builtin_convertvector(dO[s], f32x8));
+        }
+        delta += other_half(delta);
+        if (!row) delta = 0.f;
+        const int64_t at = ((int64_t)w.b * Hq + h) * p.Tq + t;
+        if (row) {
+            const float lse = p.lse[at];
+            if (lse != -INFINITY) lse2 = lse * LOG2E;
+        }
+        if (r < M && half == 0 && split == 0) p.aux[at] = delta;
+    }
+#pragma unroll
+    for (int d = 0; d < DP / 32; ++d) dQ[d] = f32x16{};
+
+    const T* k = (const T*)p.k + w.b * p.ks[0] + w.hk * p.ks[2];
+    const T* v = (const T*)p.v + w.b * p.vs[0] + w.hk * p.vs[2];
+    const int per = ((w.klen + KT - 1) / KT + p.nsplit - 1) / p.nsplit * KT;
+    const int kbeg = split * per, kend = row_time(p, w.tile * 128) < w.qlen ? min(w.klen, kbeg + per) : kbeg;
+    const int nt = kend > kbeg ? (kend - kbeg + KT - 1) / KT : 0;
+    Stage<T, DP, KT, 256> sk, sv;
+    uint64_t bits = 0, next = 0;
+    auto fetch = [&](int j) {
+        const int key0 = kbeg + j * KT, last = kend - 1;
+        next = key_bits(p, w, key0, kend, lane) & 0xffffffffull;
+        sk.load([&](int i) { return k + (int64_t)min(key0 + i, last) * p.ks[1]; }, p.D, tid);
+        sv.load([&](int i) { return v + (int64_t)min(key0 + i, last) * p.vs[1]; }, p.D, tid);
+    };
+    auto commit = [&](int j) {
+        char* x = lds + (j & 1) * 2 * TB;
+        sk.store(x, next, p.D, tid);
+        sv.store(x + TB, next, p.D, tid);
+        bits = next;
+    };
+    if (nt) { fetch(0); commit(0); }
+    for (int j = 0; j < nt; ++j) {
+        const uint64_t now = bits;
+        __syncthreads();
+        if (j + 1 < nt) fetch(j + 1);
+        if (now) {
+            const char *tk = lds + (j & 1) * 2 * TB, *tv = tk + TB;
+            f32x16 S = {}, dP = {};
+#pragma unroll
+            for (int s = 0; s < DP / 16; ++s) {
+                S = El<T>::mma(row_frag<T, DP>(tk, 0, s, lane), Q[s], S);
+                dP = El<T>::mma(row_frag<T, DP>(tv, 0, s, lane), dO[s], dP);
+            }
+            const uint32_t b = (uint32_t)now >> (4 * half);
+#pragma unroll
+            for (int i = 0; i < 16; ++i) {
+                const float x = exp2_(fmaf(S[i], c, -lse2)) * (dP[i] - delta);
+                S[i] = now == 0xffffffffull || ((b >> (8 * (i / 4) + i % 4)) & 1) ? x : 0.f;
+            }
+#pragma unroll
+            for (int s = 0; s < 2; ++s) {
+                const frag_t<T> dS = next_frag<T>(S, s);
+#pragma unroll
+                for (int d = 0; d < DP / 32; ++d) dQ[d] = El<T>::mma(trans_frag<T, DP>(tk, 16 * s, 32 * d, lane), dS, dQ[d]);
+            }
+        }
+        if (j + 1 < nt) commit(j + 1);
+    }
+
+    if (r < M) {
+        const int64_t at = (((int64_t)w.b * p.Tq + t) * Hq + h) * p.D;
+        T* o = (T*)p.o0 + at;
+        float* part = p.part + (int64_t)split * p.B * p.Tq * Hq * p.D + at;
+#pragma unroll
+        for (int d = 0; d < DP / 32; ++d)
+#pragma unroll
+            for (int g = 0; g < 4; ++g) {
+                const int e = 32 * d + 8 * g + 4 * half;
+                f32x4 x = {dQ[d][4 * g], dQ[d][4 * g + 1], dQ[d][4 * g + 2], dQ[d][4 * g + 3]};
+                x = row ? x * p.scale : f32x4{0.f, 0.f, 0.f, 0.f};
+                if (e < p.D) {
+                    if (p.nsplit == 1) store4<T>(o + e, x);
+                    else *(f32x4*)(part + e) = x;
+                }
+            }
+    }
+}
+
+// ---- dk, dv: S = q K^T and dP = dout V^T have the keys as columns; P and dS are the operands of dv^T = dout^T P and dk^T = q^T dS.
+// BOTH: one workgroup forms both.  Otherwise (D > 128: both results and both key operands do not fit the registers) half of the grid
+// forms dv and half dk, and the scores are formed twice. ----
+template <class T, int DP, bool BOTH>
+__global__ __launch_bounds__(256) void attn_dkv(const AttnP p) {
+    constexpr int RT = 32, TB = Tile<T, DP>::bytes(RT), NACC = BOTH ? 2 : 1;
+    __shared__ __attribute__((aligned(16))) char lds[4 * TB];
+    __shared__ __attribute__((aligned(16))) float stat[2][2][RT];       // lse (units of log2) and delta of a tile's rows
+    const int tid = threadIdx.x, lane = tid & 63, wave = tid >> 6, half = lane >> 5, col = lane & 31;
+    const int Hq = p.Hk * p.G, tiles = (p.Tk + 127) / 128;
+    int lin = on_xcd(blockIdx.x, tiles * p.B * p.Hk * p.nsplit * (BOTH ? 1 : 2));
+    const bool want_dk = !BOTH && (lin & 1);                              // !BOTH: this workgroup's job
+    if (!BOTH) lin >>= 1;
+    const int split = lin % p.nsplit;
+    const Where w = where(p, lin / p.nsplit, tiles);
+    const int key = w.tile * 128 + wave * 32 + col;
+    const bool ok = (key_bits(p, w, w.tile * 128 + wave * 32, w.klen, lane) >> col) & 1;
+    const float c = p.scale * LOG2E;
+
+    frag_t<T> K[DP / 16], V[DP / 16];
+    f32x16 acc[NACC][DP / 32];                                            // dv first
+    const int64_t kk = min(key, p.Tk - 1);
+    row_frags<T, DP>(K, (const T*)p.k + w.b * p.ks[0] + w.hk * p.ks[2] + kk * p.ks[1], p.D, ok, half);
+    if (BOTH || want_dk) row_frags<T, DP>(V, (const T*)p.v + w.b * p.vs[0] + w.hk * p.vs[2] + kk * p.vs[1], p.D, ok, half);
+#pragma unroll
+    for (int a = 0; a < NACC; ++a)
+#pragma unroll
+        for (int d = 0; d < DP / 32; ++d) acc[a][d] = f32x16{};
+
+    const int rows = w.tile * 128 < w.klen ? w.qlen * p.G : 0;
+    const int per = ((rows + RT - 1) / RT + p.nsplit - 1) / p.nsplit * RT;
+    const int rbeg = split * per, rend = min(rows, rbeg + per);
+    const int nt = rend > rbeg ? (rend - rbeg + RT - 1) / RT : 0;
+    Stage<T, DP, RT, 256> sq, so;
+    float lse2 = INFINITY, delta = 0.f;
+    auto fetch = [&](int j) {
+        const int r0 = rbeg + j * RT;
+        sq.load([&](int i) { return row_ptr<T>(p, p.q, w, r0 + i, p.qs[0], p.qs[1], p.qs[2]); }, p.D, tid);
+        so.load([&](int i) { return row_ptr<T>(p, p.dout, w, r0 + i, p.ds[0], p.ds[1], p.ds[2]); }, p.D, tid);
+        if (tid < RT) {
+            const int r = r0 + tid, t = row_time(p, r);
+            lse2 = INFINITY;
+            delta = 0.f;
+            if (r < rend) {
+                const int64_t at = ((int64_t)w.b * Hq + w.hk * p.G + r - t * p.G) * p.Tq + t;
+                const float lse = p.lse[at];
+                if (lse != -INFINITY) lse2 = lse * LOG2E;
+                delta = p.aux[at];
+            }
+        }
+    };
+    auto commit = [&](int j) {
+        char* x = lds + (j & 1) * 2 * TB;
+        const int left = rend - (rbeg + j * RT);
+        const uint64_t bits = left >= RT ? 0xffffffffull : (1ull << left) - 1;
+        sq.store(x, bits, p.D, tid);
+        so.store(x + TB, bits, p.D, tid);
+        if (tid < RT) { stat[j & 1][0][tid] = lse2; stat[j & 1][1][tid] = delta; }
+    };
+    if (nt) { fetch(0); commit(0); }
+    for (int j = 0; j < nt; ++j) {
+        __syncthreads();
+        if (j + 1 < nt) fetch(j + 1);
+        const char *tq = lds + (j & 1) * 2 * TB, *to = tq + TB;
+        f32x16 S = {};
+#pragma unroll
+        for (int s = 0; s < DP / 16; ++s) S = El<T>::mma(row_frag<T, DP>(tq, 0, s, lane), K[s], S);
+#pragma unroll
+        for (int g = 0; g < 4; ++g) {
+            const f32x4 l = *(const f32x4*)&stat[j & 1][0][8 * g + 4 * half];
+#pragma unroll
+            for (int i = 0; i < 4; ++i) S[4 * g + i] = exp2_(fmaf(S[4 * g + i], c, -l[i]));
+        }
+        if (BOTH || !want_dk) {
+#pragma unroll
+            for (int s = 0; s < 2; ++s) {
+                const frag_t<T> P = next_frag<T>(S, s);
+#pragma unroll
+                for (int d = 0; d < DP / 32; ++d) acc[0][d] = El<T>::mma(trans_frag<T, DP>(to, 16 * s, 32 * d, lane), P, acc[0][d]);
+            }
+        }
+        if (BOTH || want_dk) {
+            f32x16 dP = {};
+#pragma unroll
+            for (int s = 0; s < DP / 16; ++s) dP = El<T>::mma(row_frag<T, DP>(to, 0, s, lane), V[s], dP);
+#pragma unroll
+            for (int g = 0; g < 4; ++g) {
+                const f32x4 x = *(const f32x4*)&stat[j & 1][1][8 * g + 4 * half];
+#pragma unroll
+                for (int i = 0; i < 4; ++i) S[4 * g + i] *= dP[4 * g + i] - x[i];
+            }
+#pragma unroll
+            for (int s = 0; s < 2; ++s) {
+                const frag_t<T> dS = next_frag<T>(S, s);
+#pragma unroll
+                for (int d = 0; d < DP / 32; ++d)
+                    acc[NACC - 1][d] = El<T>::mma(trans_frag<T, DP>(tq, 16 * s, 32 * d, lane), dS, acc[NACC - 1][d]);
+            }
+        }
+        if (j + 1 < nt) commit(j + 1);
+    }
+
+    if (key < p.Tk) {
+        const int64_t n = (int64_t)p.B * p.Tk * p.Hk * p.D, at = (((int64_t)w.b * p.Tk + key) * p.Hk + w.hk) * p.D;
+#pragma unroll
+        for (int a = 0; a < NACC; ++a) {
+            const bool dk = BOTH ? a == 1 : want_dk;
+            T* o = (T*)(dk ? p.o1 : p.o0) + at;
+            float* part = p.part + ((dk ? p.nsplit : 0) + split) * n + at;
+            const float f = dk ? p.scale : 1.f;
+#pragma unroll
+            for (int d = 0; d < DP / 32; ++d)
+#pragma unroll
+                for (int g = 0; g < 4; ++g) {
+                    const int e = 32 * d + 8 * g + 4 * half;
+                    f32x4 x = {acc[a][d][4 * g], acc[a][d][4 * g + 1], acc[a][d][4 * g + 2], acc[a][d][4 * g + 3]};
+                    x = ok ? x * f : f32x4{0.f, 0.f, 0.f, 0.f};
+                    if (e < p.D) {
+                        if (p.nsplit == 1) store4<T>(o + e, x);
+                        else *(f32x4*)(part + e) = x;
+                    }
+                }
+        }
+    }
+}
+
+// out[i] = the sum of the splits' results in their order; y = 1: dk
+struct SumP { const float* part; void *o0, *o1; int64_t n; int nsplit; };
+template <class T> __global__ __launch_bounds__(256) void attn_sum(const SumP p) {
+    const int64_t i = ((int64_t)blockIdx.x * 256 + threadIdx.x) * 4;
+    if (i >= p.n) return;                                                 // n is a multiple of 8
+    const float* at = p.part + blockIdx.y * p.nsplit * p.n + i;
+    f32x4 s = *(const f32x4*)at;
+    for (int k = 1; k < p.nsplit; ++k) s += *(const f32x4*)(at + k * p.n);
+    store4<T>((T*)(blockIdx.y ? p.o1 : p.o0) + i, s);
+}
+
+// ---- host side -------------------------------------------------------------------------------------------------------------------------
+struct GradPlan { int dq_split, kv_split; int64_t dq_units, kv_units, nq, nk; bool both; };
+static int split_for(int64_t groups, int64_t pieces) {
+    const int64_t n = groups > 0 ? cdiv(512, groups) : 1;
+    const int64_t k = n < pieces ? n : pieces;
+    return (int)(k < 1 ? 1 : k > 16 ? 16 : k);
+}
+static GradPlan gradient_plan(const oph_seq_attn* a) {
+    const int64_t M = (int64_t)a->Tq * (a->Hq / a->Hk), heads = (int64_t)a->B * a->Hk;
+    GradPlan g;
+    g.both = a->D <= 128;
+    g.dq_units = cdiv(M, 128) * heads;
+    g.kv_units = cdiv(a->Tk, 128) * heads * (g.both ? 1 : 2);
+    g.dq_split = split_for(g.dq_units, cdiv(a->Tk, 128));
+    g.kv_split = split_for(g.kv_units, cdiv(M, 128));
+    g.nq = (int64_t)a->B * a->Tq * a->Hq * a->D;
+    g.nk = (int64_t)a->B * a->Tk * a->Hk * a->D;
+    return g;
+}
+static int64_t delta_floats(const oph_seq_attn* a) { return cdiv((int64_t)a->B * a->Hq * a->Tq, 4) * 4; }
+int64_t attn_gradient_workspace(const oph_seq_attn* a) {
+    const GradPlan g = gradient_plan(a);
+    const int64_t q = g.dq_split > 1 ? g.dq_split * g.nq : 0, k = g.kv_split > 1 ? 2 * g.kv_split * g.nk : 0;
+    return (delta_floats(a) + (q > k ? q : k)) * (int64_t)sizeof(float);   // the two passes use the same partial results' space in turn
+}
+
+template <class T> static int sum(const float* part, void* o0, void* o1, int64_t n, int nsplit, void* stream) {
+    const SumP s = {part, o0, o1, n, nsplit};
+    return launch<SumP>(attn_sum<T>, dim3((unsigned)cdiv(n, 1024), o1 ? 2 : 1), 256, s, 0, stream);
+}
+template <class T, int DP> static int gradient(const oph_seq_attn* a, AttnP p, void* stream) {
+    const GradPlan g = gradient_plan(a);
+    if (g.nq) {
+        p.nsplit = g.dq_split;
+        p.o0 = a->dq;
+        if (int rc = launch<AttnP>(attn_dq<T, DP>, dim3((unsigned)(g.dq_units * g.dq_split)), 256, p, 0, stream)) return rc;
+        if (g.dq_split > 1) {
+            if (int rc = sum<T>(p.part, a->dq, nullptr, g.nq, g.dq_split, stream)) return rc;
+        }
+    }
+    if (g.nk) {
+        p.nsplit = g.kv_split;
+        p.o0 = a->dv;
+        p.o1 = a->dk;
+        if (int rc = launch<AttnP>(attn_dkv<T, DP, DP <= 128>, dim3((unsigned)(g.kv_units * g.kv_split)), 256, p, 0, stream)) return rc;
+        if (g.kv_split > 1) return sum<T>(p.part, a->dv, a->dk, g.nk, g.kv_split, stream);
+    }
+    return OPH_OK;
+}
+template <class T> static int gradient_d(const oph_seq_attn* a, const AttnP& p, void* stream) {
+    if (p.D <= 64) return gradient<T, 64>(a, p, stream);
+    if (p.D <= 128) return gradient<T, 128>(a, p, stream);
+    return gradient<T, 256>(a, p, stream);
+}
+
+}  // namespace ophseq
+
+using namespace ophseq;
+extern "C" int oph_seq_attn_gradient(const oph_seq_attn* a, int device, void* stream) {
+    if (int rc = attn_check(a, true)) return rc;
+    if (!a->B || (!a->Tq && !a->Tk)) return OPH_OK;
+    if (a->Tq && (!a->q || !a->out || !a->lse || !a->dout || !a->dq)) return fail(OPH_ERR_INVALID, "attention: q, out, lse, dout and dq must not be NULL");
+    if (a->Tk && (!a->k || !a->v || !a->dk || !a->dv)) return fail(OPH_ERR_INVALID, "attention: k, v, dk and dv must not be NULL");
+    const int64_t need = attn_gradient_workspace(a);
+    if (need && (!a->workspace || (int64_t)a->workspace_bytes < need || ((uintptr_t)a->workspace & 15)))
+        return fail(OPH_ERR_INVALID, "attention: the workspace must hold %lld bytes, 16-byte aligned", (long long)need);
+    OnDevice on(device);
+    if (on.status) return on.status;
+    AttnP p = attn_params(a);
+    p.out = a->out;
+    p.dout = a->dout;
+    p.lse = a->lse;
+    p.aux = (float*)a->workspace;
+    p.part = p.aux + delta_floats(a);
+    for (int i = 0; i < 3; ++i) p.ds[i] = a->dout_stride[i];
+    if (a->dtype == OPH_SEQ_F32) return gradient_d<float>(a, p, stream);
+    if (a->dtype == OPH_SEQ_BF16) return gradient_d<bf16_t>(a, p, stream);
+    return gradient_d<f16_t>(a, p, stream);
+}

@@ -1,0 +1,333 @@
+// Embedding lookup with scaling, and its gradient by sorted tokens: oph_seq_embed_lookup, oph_seq_embed_gradient.
+//
+// Gradient.  embed_order lists the positions of every table row in ascending order, row after row (a stable sort by row, in one
+// launch): each workgroup owns one bucket of rows (row mod buckets), reads all ids twice from the L2 -- once to count, once to
+// place -- and learns from the same counting how many tokens lie in the buckets before its own.  embed_sum walks the sorted tokens in
+// pieces of CHUNK, one run of equal rows after the other; a run inside a piece goes straight to the gradient, what crosses a border is
+// left in `part` and summed by embed_join in the order of the pieces.  No floating-point atomics: the sums run in a fixed order.
+#include "oph_seq.h"
+#include "../../include/ophelia_hip.h"
+
+#include <algorithm>
+
+namespace ophseq {
+
+constexpr int CHUNK = 32, WAVES = 16, LOCAL = 1024;       // tokens of a piece | waves of embed_order, most rows of its bucket
+
+struct EmbedP {
+    const void *ids, *src;          // src: table or dout
+    void* out;                      // rows or gradient
+    int* head;                      // [0]: number of sorted tokens, from [4] on: their positions, then their rows
+    float* part;                    // [piece][begun before | goes on][U4]
+    int64_t n, stride;
+    int vocab, units, u4, zero_pad, lpr, buckets, shift;
+    float scale;
+};
+
+// the row that token i names; -1: none
+template <class I> __device__ __forceinline__ int row_of(const EmbedP& p, int64_t i) {
+    const int64_t id = ((const I*)p.ids)[i];
+    return id < 0 || id >= p.vocab || (id == 0 && p.zero_pad) ? -1 : (int)id;
+}
+
+// PER16 consecutive elements of a row as floats; `left` elements remain in the row
+template <class T> __device__ __forceinline__ void load_piece(float (&x)[El<T>::PER16], const T* at, int left) {
+    constexpr int PER = El<T>::PER16;
+    typedef T vec __attribute__((ext_vector_type(PER)));
+    if (left >= PER) {
+        const vec v = __builtin_bit_cast(vec, load16(at));
+#pragma unroll
+        for (int j = 0; j < PER; ++j) x[j] = (float)v[j];
+    } else {
+#pragma unroll
+        for (int j = 0; j < PER; ++j) x[j] = j < left ? (float)at[j] : 0.f;
+    }
+}
+template <class T> __device__ __forceinline__ void store_piece(T* at, const float (&x)[El<T>::PER16], int left) {
+    constexpr int PER = El<T>::PER16;
+    typedef T vec __attribute__((ext_vector_type(PER)));
+    if (left >= PER) {
+        vec v;
+#pragma unroll
+        for (int j = 0; j < PER; ++j) v[j] = (T)x[j];
+        store16(at, __builtin_bit_cast(u32x4, v));
+    } else {
+#pragma unroll
+        for (int j = 0; j < PER; ++j)
+            if (j < left) at[j] = (T)x[j];
+    }
+}
+
+// lpr lanes (a power of two) copy a row, 16 bytes at a time
+template <class T, class I> __global__ __launch_bounds__(256) void embed_lookup(const EmbedP p) {
+    constexpr int PER = El<T>::PER16;
+    const int lane = threadIdx.x & (p.lpr - 1);
+    const int64_t i = (int64_t)blockIdx.x * (256 / p.lpr) + threadIdx.x / p.lpr;
+    if (i >= p.n) return;
+    const int row = row_of<I>(p, i);
+    const T* from = (const T*)p.src + (row < 0 ? 0 : row) * p.stride;
+    T* to = (T*)p.out + i * p.units;
+    for (int c = lane * PER; c < p.units; c += p.lpr * PER) {
+        float x[PER];
+        if (row >= 0) load_piece<T>(x, from + c, p.units - c);
+#pragma unroll
+        for (int j = 0; j < PER; ++j) x[j] = row >= 0 ? x[j] * p.scale : 0.f;
+        store_piece<T>(to + c, x, p.units - c);
+    }
+}
+
+// bucket b = blockIdx.x holds rows b, b + buckets, ...; the row's number inside it is row >> shift
+template <class T, class I> __global__ __launch_bounds__(64 * WAVES) void embed_order(const EmbedP p) {
+    __shared__ int count[WAVES][LOCAL];
+    __shared__ int wsum[WAVES], wless[WAVES];
+    const int tid = threadIdx.x, lane = tid & 63, wave = tid >> 6, bucket = blockIdx.x;
+    const int local = (p.vocab - bucket + p.buckets - 1) >> p.shift;            // rows of this bucket, at most LOCAL
+    for (int i = tid; i < WAVES * LOCAL; i += 64 * WAVES) (&count[0][0])[i] = 0;
+    __syncthreads();
+    const int64_t per = (p.n + 64 * WAVES - 1) / (64 * WAVES) * 64;
+    const int64_t beg = wave * per, end = std::min(p.n, beg + per);
+    int less = 0;
+#pragma unroll 4
+    for (int64_t i = beg + lane; i < end; i += 64) {
+        const int row = row_of<I>(p, i), b = row & (p.buckets - 1);
+        if (row >= 0) {
+            less += b < bucket;
+            if (b == bucket) atomicAdd(&count[wave][row >> p.shift], 1);
+        }
+    }
+#pragma unroll
+    for (int i = 32; i; i >>= 1) less += __shfl_xor(less, i);
+    if (lane == 0) wless[wave] = less;
+    __syncthreads();
+    // exclusive sums over (row, wave): thread = row
+    int own = 0;
+    if (tid < local)
+        for (int w = 0; w < WAVES; ++w) own += count[w][tid];
+    int run = own;
+#pragma unroll
+    for (int i = 1; i < 64; i <<= 1) {
+        const int x = __shfl_up(run, i);
+        if (lane >= i) run += x;
+    }
+    if (lane == 63) wsum[wave] = run;
+    __syncthreads();
+    int base = 0;
+    for (int w = 0; w < WAVES; ++w) base += wless[w] + (w < wave ? wsum[w] : 0);
+    int at = base + run - own;
+    if (tid < local)
+        for (int w = 0; w < WAVES; ++w) {
+            const int c = count[w][tid];
+            count[w][tid] = at;
+            at += c;
+        }
+    if (bucket == p.buckets - 1 && tid == 64 * WAVES - 1) p.head[0] = at;       // the last thread's end is the end of all
+    __syncthreads();
+    int *pos = p.head + 4, *key = pos + p.n;
+    for (int64_t i = beg + lane; i < beg + per; i += 64) {                      // beg + per: whole waves take part in the ballots
+        const int row = i < end ? row_of<I>(p, i) : -1;
+        const bool mine = row >= 0 && (row & (p.buckets - 1)) == bucket;
+        uint64_t todo = __ballot(mine);
+        while (todo) {
+            const int leader = __ffsll((unsigned long long)todo) - 1;
+            const int r = __builtin_amdgcn_readlane(row, leader);
+            const uint64_t same = __ballot(mine && row == r);
+            const int first = count[wave][r >> p.shift];
+            if (mine && row == r) {
+                const int to = first + __popcll(same & ((1ull << lane) - 1));
+                pos[to] = (int)i;
+                key[to] = r;
+            }
+            if (lane == leader) count[wave][r >> p.shift] = first + __popcll(same);
+            __builtin_amdgcn_fence(__ATOMIC_RELEASE, "wavefront");
+            __builtin_amdgcn_wave_barrier();
+            __builtin_amdgcn_fence(__ATOMIC_ACQUIRE, "wavefront");
+            todo &= ~same;
+        }
+    }
+    __syncthreads();
+    // rows that no token names.  count[w][r] now is the end of wave w's tokens of row r: a row is empty where the last wave's end is
+    // the end of the row before
+    constexpr int PER = El<T>::PER16;
+    for (int r = wave; r < local; r += WAVES) {
+        int beg = 0;
+        if (r > 0) beg = count[WAVES - 1][r - 1];
+        else
+            for (int w = 0; w < WAVES; ++w) beg += wless[w];
+        if (count[WAVES - 1][r] != beg) continue;
+        T* to = (T*)p.out + (((int64_t)r << p.shift) + bucket) * p.units;
+        const float zero[PER] = {};
+        for (int c = lane * PER; c < p.units; c += 64 * PER) store_piece<T>(to + c, zero, p.units - c);
+    }
+}
+
+// lpr lanes per (piece, lpr * PER16 channels)
+template <class T> __global__ __launch_bounds__(256) void embed_sum(const EmbedP p) {
+    constexpr int PER = El<T>::PER16, AHEAD = 8;
+    const int lane = threadIdx.x & (p.lpr - 1), count = p.head[0];
+    const int64_t piece = (int64_t)blockIdx.x * (256 / p.lpr) + threadIdx.x / p.lpr;
+    const int c = (blockIdx.y * p.lpr + lane) * PER, left = p.units - c;
+    if (piece * CHUNK >= count || left <= 0) return;
+    const int *pos = p.head + 4, *key = pos + p.n;
+    const int beg = (int)piece * CHUNK, end = min(count, beg + CHUNK);
+    const T* src = (const T*)p.src + c;
+    int cur = key[beg];
+    bool begun = beg > 0 && key[beg - 1] == cur;
+    const int after = end < count ? key[end] : -1;
+    float acc[PER] = {};
+    auto flush = [&](bool goes_on) {
+        if (begun || goes_on) {
+            float* to = p.part + (piece * 2 + (begun ? 0 : 1)) * p.u4 + c;
+#pragma unroll
+            for (int j = 0; j < PER; j += 4)
+                if (j < left) *(f32x4*)(to + j) = f32x4{acc[j], acc[j + 1], acc[j + 2], acc[j + 3]};   // u4 is left rounded up to 4
+        } else {
+            float x[PER];
+#pragma unroll
+            for (int j = 0; j < PER; ++j) x[j] = acc[j] * p.scale;
+            store_piece<T>((T*)p.out + (int64_t)cur * p.units + c, x, left);
+        }
+    };
+    for (int i = beg; i < end; i += AHEAD) {
+        float x[AHEAD][PER];
+        int row[AHEAD];
+#pragma unroll
+        for (int a = 0; a < AHEAD; ++a) {
+            const int k = min(i + a, end - 1);
+            row[a] = key[k];
+            load_piece<T>(x[a], src + (int64_t)pos[k] * p.stride, left);
+        }
+#pragma unroll
+        for (int a = 0; a < AHEAD; ++a) {
+            if (i + a >= end) break;
+            if (row[a] != cur) {
+                flush(false);
+                cur = row[a];
+                begun = false;
+#pragma unroll
+                for (int j = 0; j < PER; ++j) acc[j] = 0.f;
+            }
+#pragma unroll
+            for (int j = 0; j < PER; ++j) acc[j] += x[a][j];
+        }
+    }
+    flush(cur == after);
+}
+
+// a workgroup per piece in which a run begins that goes on in the next: its parts, every fourth by one wave, then the four sums
+template <class T> __global__ __launch_bounds__(256) void embed_join(const EmbedP p) {
+    __shared__ f32x4 sums[4][64];
+    const int lane = threadIdx.x & 63, wave = threadIdx.x >> 6, count = p.head[0];
+    const int64_t piece = blockIdx.x, beg = piece * CHUNK, end = beg + CHUNK;
+    if (end >= count) return;                                                   // the last piece's runs end in it
+    const int *key = p.head + 4 + p.n, row = key[end - 1];
+    if (key[end] != row || (beg > 0 && key[beg - 1] == row)) return;             // ends here, or began before: row fills the piece then
+    const int c = (blockIdx.y * 64 + lane) * 4;
+    const float* at = p.part + c;
+    f32x4 s = {0.f, 0.f, 0.f, 0.f};
+    if (c < p.u4) {
+        if (wave == 0) s = *(const f32x4*)(at + (piece * 2 + 1) * p.u4);
+#pragma unroll 4
+        for (int64_t q = piece + 1 + wave; q * CHUNK < count && key[q * CHUNK] == row; q += 4) s += *(const f32x4*)(at + q * 2 * p.u4);
+    }
+    sums[wave][lane] = s;
+    __syncthreads();
+    if (wave == 0 && c < p.units) {
+        s = sums[0][lane];
+#pragma unroll
+        for (int w = 1; w < 4; ++w) s += sums[w][lane];
+        T* to = (T*)p.out + (int64_t)row * p.units + c;
+#pragma unroll
+        for (int j = 0; j < 4; ++j)
+            if (c + j < p.units) to[j] = (T)(s[j] * p.scale);
+    }
+}
+
+// ---- host side ---------------------------------------------------------------------------------------------------------------------------
+static int check(const void* ids, int id_bytes, int64_t n, int64_t stride, int vocab, int units, float scale, int dtype, const char* what) {
+    if (!type_bytes(dtype)) return fail(OPH_ERR_INVALID, "%s: dtype %d is not one of OPH_SEQ_*", what, dtype);
+    if (id_bytes != 4 && id_bytes != 8) return fail(OPH_ERR_INVALID, "%s: ids of %d bytes (4 or 8)", what, id_bytes);
+    if (n < 0 || n > 2147483647 - 4096) return fail(OPH_ERR_INVALID, "%s: %lld ids", what, (long long)n);
+    if (vocab < 1 || vocab > 1 << 28 || units < 1 || units > 1 << 24) return fail(OPH_ERR_INVALID, "%s: table of %d rows of %d", what, vocab, units);
+    if (stride < 0) return fail(OPH_ERR_INVALID, "%s: negative stride", what);
+    if (n && !ids) return fail(OPH_ERR_INVALID, "%s: ids must not be NULL", what);
+    if (!(scale - scale == 0.f)) return fail(OPH_ERR_INVALID, "%s: scale %g is not finite", what, (double)scale);
+    return OPH_OK;
+}
+static int lanes_for(int units, int dtype) {
+    const int pieces = (int)cdiv(units, 16 / type_bytes(dtype));
+    int l = 1;
+    while (l < pieces && l < 64) l *= 2;
+    return l;
+}
+static int bucket_count(int vocab) {
+    int b = 1;
+    while ((b < 256 && b < vocab) || (int64_t)b * LOCAL < vocab) b *= 2;
+    return b;
+}
+static int64_t part_offset(int64_t n) { return cdiv((4 + 2 * n) * 4, 16) * 16; }
+
+template <class T, class I> static int lookup(const EmbedP& p, void* stream) {
+    return launch<EmbedP>(embed_lookup<T, I>, dim3((unsigned)cdiv(p.n, 256 / p.lpr)), 256, p, 0, stream);
+}
+template <class T, class I> static int gradient(const EmbedP& p, void* stream) {
+    if (int rc = launch<EmbedP>(embed_order<T, I>, dim3(p.buckets), 64 * WAVES, p, 0, stream)) return rc;
+    if (!p.n) return OPH_OK;
+    const int64_t pieces = cdiv(p.n, CHUNK);
+    if (int rc = launch<EmbedP>(embed_sum<T>, dim3((unsigned)cdiv(pieces, 256 / p.lpr), (unsigned)cdiv(p.units, p.lpr * El<T>::PER16)), 256, p, 0, stream))
+        return rc;
+    if (pieces == 1) return OPH_OK;
+    return launch<EmbedP>(embed_join<T>, dim3((unsigned)pieces, (unsigned)cdiv(p.units, 256)), 256, p, 0, stream);
+}
+template <class T> static int lookup_i(const EmbedP& p, int id_bytes, void* s) { return id_bytes == 4 ? lookup<T, int32_t>(p, s) : lookup<T, int64_t>(p, s); }
+template <class T> static int gradient_i(const EmbedP& p, int id_bytes, void* s) { return id_bytes == 4 ? gradient<T, int32_t>(p, s) : gradient<T, int64_t>(p, s); }
+
+}  // namespace ophseq
+
+using namespace ophseq;
+extern "C" {
+
+int oph_seq_embed_lookup(const void* ids, int id_bytes, int64_t n, const void* table, int64_t table_stride, int vocab, int units, float scale,
+                         int zero_pad, int dtype, void* out, int device, void* stream) {
+    if (int rc = check(ids, id_bytes, n, table_stride, vocab, units, scale, dtype, "embedding lookup")) return rc;
+    if (!n) return OPH_OK;
+    if (!table || !out) return fail(OPH_ERR_INVALID, "embedding lookup: table and out must not be NULL");
+    OnDevice on(device);
+    if (on.status) return on.status;
+    EmbedP p = {};
+    p.ids = ids; p.src = table; p.out = out; p.n = n; p.stride = table_stride; p.vocab = vocab; p.units = units; p.zero_pad = zero_pad != 0;
+    p.lpr = lanes_for(units, dtype);
+    p.scale = scale;
+    if (dtype == OPH_SEQ_F32) return lookup_i<float>(p, id_bytes, stream);
+    if (dtype == OPH_SEQ_BF16) return lookup_i<bf16_t>(p, id_bytes, stream);
+    return lookup_i<f16_t>(p, id_bytes, stream);
+}
+
+int64_t oph_seq_embed_workspace(int64_t n, int vocab, int units) {
+    if (int rc = check(&n, 4, n, 0, vocab, units, 1.f, OPH_SEQ_F32, "embedding gradient")) return rc;
+    return part_offset(n) + cdiv(n, CHUNK) * 2 * cdiv(units, 4) * 16;
+}
+
+int oph_seq_embed_gradient(const void* ids, int id_bytes, int64_t n, const void* dout, int64_t dout_stride, int vocab, int units, float scale,
+                           int zero_pad, int dtype, void* grad, void* workspace, size_t workspace_bytes, int device, void* stream) {
+    if (int rc = check(ids, id_bytes, n, dout_stride, vocab, units, scale, dtype, "embedding gradient")) return rc;
+    if (!grad || (n && !dout)) return fail(OPH_ERR_INVALID, "embedding gradient: dout and grad must not be NULL");
+    const int64_t need = oph_seq_embed_workspace(n, vocab, units);
+    if (!workspace || (int64_t)workspace_bytes < need || ((uintptr_t)workspace & 15))
+        return fail(OPH_ERR_INVALID, "embedding gradient: the workspace must hold %lld bytes, 16-byte aligned", (long long)need);
+    OnDevice on(device);
+    if (on.status) return on.status;
+    EmbedP p = {};
+    p.ids = ids; p.src = dout; p.out = grad; p.n = n; p.stride = dout_stride; p.vocab = vocab; p.units = units; p.zero_pad = zero_pad != 0;
+    p.u4 = (int)cdiv(units, 4) * 4;
+    p.lpr = lanes_for(units, dtype);
+    p.scale = scale;
+    p.buckets = bucket_count(vocab);
+    while ((1 << p.shift) < p.buckets) ++p.shift;
+    p.head = (int*)workspace;
+    p.part = (float*)((char*)workspace + part_offset(n));
+    if (dtype == OPH_SEQ_F32) return gradient_i<float>(p, id_bytes, stream);
+    if (dtype == OPH_SEQ_BF16) return gradient_i<bf16_t>(p, id_bytes, stream);
+    return gradient_i<f16_t>(p, id_bytes, stream);
+}
+
+}  // extern "C"

@@ -2,12 +2,15 @@
 conv1d 91-146, hc 148-207, conv1d_transpose 209-258) plus networks.Attention
 (networks.py:286-325, monotonic branch).  Same names, argument meaning and (B,T,C)
 layout; variables come from a dict keyed by the TF variable names under `scope`.
-Every function executes on the GPU through the per-operator C-ABI entry points."""
+Every function executes on the GPU through the per-operator C-ABI entry points.
+The operators of device_ops (torch tensors on the GPU, with gradients) are offered here as well."""
 import ctypes as C
 
 import numpy as np
 
 from . import _lib
+from .device_ops import (cross_attention, cross_attention_gradient, embed_gradient, embed_lookup, gated_recurrence,  # noqa: F401
+                         gated_recurrence_gradient)
 
 _ACT = {None: 0, "relu": 1, "sigmoid": 2}
 _PAD = {"same": 0, "causal": 1}

@@ -1,0 +1,119 @@
+"""libophelia_seq.so without a GPU: it exports what include/ophelia_seq.h declares, refuses bad arguments before it looks for a device, and
+fails loudly where there is none."""
+import ctypes as C
+import os
+import re
+
+import pytest
+import torch
+
+from conftest import ROOT
+
+
+@pytest.fixture(scope="module")
+def lib():
+    from ophelia_amd import _lib
+    if not os.path.exists(_lib.SEQ_LIBPATH):
+        _lib.build()
+    return _lib.load_seq()
+
+
+def test_library_exports_every_declared_symbol(lib):
+    from ophelia_amd import _lib
+    txt = re.sub(r"/\*.*?\*/", "", open(os.path.join(ROOT, "include", "ophelia_seq.h")).read(), flags=re.S)
+    syms = set(re.findall(r"\b(oph_seq_[a-z0-9_]+)\s*\(", txt))
+    assert syms == set(_lib.SEQ_SIGNATURES)
+    assert lib.oph_seq_abi_version() == 1
+
+
+def _attn(**over):
+    from ophelia_amd import _lib
+    a = _lib.OphSeqAttn()
+    for n in ("q", "k", "v", "out", "lse", "dout", "dq", "dk", "dv"):
+        setattr(a, n, 4096)                      # never followed: every call below is refused
+    a.B, a.Tq, a.Tk, a.Hq, a.Hk, a.D, a.dtype, a.scale = 2, 3, 5, 4, 2, 64, 1, 0.125
+    for n, x in over.items():
+        setattr(a, n, x)
+    return a
+
+
+@pytest.mark.parametrize("over,word", [(dict(dtype=3), "dtype"), (dict(B=-1), "negative"), (dict(Tk=-1), "negative"), (dict(Hq=3), "multiple"),
+                                       (dict(Hk=0), "multiple"), (dict(D=12), "head size"), (dict(D=264), "head size"), (dict(D=0), "head size"),
+                                       (dict(scale=0.0), "scale"), (dict(scale=-1.0), "scale"), (dict(scale=float("nan")), "scale"),
+                                       (dict(scale=float("inf")), "scale"), (dict(Tq=2 ** 31 - 1), "too many"), (dict(q=None), "NULL"),
+                                       (dict(k=None), "NULL"), (dict(out=None), "NULL"), (dict(Tk=100000, Tq=1), "workspace"),
+                                       (dict(Tk=100000, Tq=1, workspace=4096, workspace_bytes=64), "workspace"),
+                                       (dict(Tk=100000, Tq=1, workspace=4100, workspace_bytes=1 << 40), "workspace")], ids=str)
+def test_attention_refusals(lib, over, word):
+    a = _attn(**over)
+    for call in (lib.oph_seq_attn_forward, lib.oph_seq_attn_gradient):
+        rc = call(C.byref(a), 0, None)
+        assert rc in (-1, -4) and word in lib.oph_seq_last_error().decode(), (rc, lib.oph_seq_last_error())
+    if word in ("dtype", "negative", "multiple", "head size", "scale", "too many"):
+        assert lib.oph_seq_attn_workspace(C.byref(a), 0) < 0
+
+
+def test_empty_calls_and_null_arguments(lib):
+    assert lib.oph_seq_attn_forward(None, 0, None) == -1 and lib.oph_seq_recur_forward(None, 0, None) == -1
+    a = _attn(B=0)
+    assert lib.oph_seq_attn_forward(C.byref(a), 0, None) == 0 and lib.oph_seq_attn_gradient(C.byref(a), 0, None) == 0
+    assert lib.oph_seq_embed_lookup(None, 4, 0, None, 8, 5, 8, 1.0, 1, 0, None, 0, None) == 0
+
+
+@pytest.mark.parametrize("args,word", [((4096, 2, 5, 4096, 8, 5, 8, 1.0, 1, 0), "bytes"), ((4096, 4, -1, 4096, 8, 5, 8, 1.0, 1, 0), "ids"),
+                                       ((4096, 4, 5, 4096, 8, 0, 8, 1.0, 1, 0), "table"), ((4096, 4, 5, 4096, 8, 5, 0, 1.0, 1, 0), "table"),
+                                       ((4096, 4, 5, 4096, -8, 5, 8, 1.0, 1, 0), "stride"), ((4096, 4, 5, 4096, 8, 5, 8, float("nan"), 1, 0), "scale"),
+                                       ((4096, 4, 5, 4096, 8, 5, 8, 1.0, 1, 9), "dtype"), ((None, 4, 5, 4096, 8, 5, 8, 1.0, 1, 0), "NULL"),
+                                       ((4096, 4, 5, None, 8, 5, 8, 1.0, 1, 0), "NULL")], ids=str)
+def test_embedding_refusals(lib, args, word):
+    assert lib.oph_seq_embed_lookup(*args, 4096, 0, None) == -1 and word in lib.oph_seq_last_error().decode()
+    assert lib.oph_seq_embed_gradient(*args, 4096, 4096, 1 << 40, 0, None) == -1 and word in lib.oph_seq_last_error().decode()
+
+
+def test_embedding_workspace_is_checked(lib):
+    ok = (4096, 4, 500, 4096, 8, 5, 8, 1.0, 1, 0, 4096)
+    need = lib.oph_seq_embed_workspace(500, 5, 8)
+    for ws, size in ((None, need), (4096, need - 1), (4104, need)):
+        assert lib.oph_seq_embed_gradient(*ok, ws, size, 0, None) == -1 and "workspace" in lib.oph_seq_last_error().decode()
+
+
+@pytest.mark.parametrize("over,word", [(dict(dtype=-1), "dtype"), (dict(B=-1), "size"), (dict(T=-1), "size"), (dict(C=0), "size"), (dict(x=None), "NULL"),
+                                       (dict(gate=None), "NULL"), (dict(h=None), "NULL"), (dict(T=2 ** 31 - 1), "too large")], ids=str)
+def test_recurrence_refusals(lib, over, word):
+    from ophelia_amd import _lib
+    a = _lib.OphSeqRecur()
+    for n in ("x", "gate", "h", "h_last", "dh", "dx", "dgate"):
+        setattr(a, n, 4096)
+    a.B, a.T, a.C, a.dtype = 2, 3, 4, 0
+    for n, v in over.items():
+        setattr(a, n, v)
+    for call in (lib.oph_seq_recur_forward, lib.oph_seq_recur_gradient):
+        assert call(C.byref(a), 0, None) in (-1, -4) and word in lib.oph_seq_last_error().decode()
+
+
+def test_no_cpu_fallback():
+    from ophelia_amd import modules as M
+    q = torch.zeros(1, 2, 1, 8)
+    for call in (lambda: M.cross_attention(q, q, q), lambda: M.embed_lookup(torch.zeros(3, dtype=torch.int32), torch.zeros(4, 4)),
+                 lambda: M.embed_gradient(torch.zeros(3, dtype=torch.int32), torch.zeros(3, 4), 4),
+                 lambda: M.gated_recurrence(torch.zeros(1, 2, 3), torch.zeros(1, 2, 3)),
+                 lambda: M.cross_attention_gradient(q, q, q, q, q, torch.zeros(1, 1, 2)),
+                 lambda: M.gated_recurrence_gradient(*[torch.zeros(1, 2, 3)] * 4)):
+        with pytest.raises(ValueError, match="GPU only"):
+            call()
+    with pytest.raises(ValueError, match="float32, bfloat16 or float16"):
+        M.cross_attention(q.double(), q.double(), q.double())
+
+
+def test_without_a_device_the_library_says_so(lib):
+    if torch.cuda.is_available():
+        pytest.skip("GPU present")
+    a = _attn()
+    assert lib.oph_seq_attn_forward(C.byref(a), 0, None) == -3 and "HIP device" in lib.oph_seq_last_error().decode()
+
+
+def test_product_sources_of_the_operators_stand_alone():
+    """no oracle, and packed float32 instructions switched off for this library (some of their forms have given wrong results)"""
+    src = open(os.path.join(ROOT, "ophelia_amd", "device_ops.py")).read()
+    assert "oracle" not in src
+    assert "-packed-fp32-ops" in open(os.path.join(ROOT, "ophelia_amd", "_lib.py")).read()
