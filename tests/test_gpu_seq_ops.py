@@ -244,7 +244,7 @@ def test_embed_strides_and_far_rows():
 
 # ---- gated linear recurrence ---------------------------------------------------------------------------------------------------------
 @dtypes
-@pytest.mark.parametrize("B,T,C", [(1, 1, 1), (2, 1, 256), (3, 7, 5), (16, 200, 256), (2, 257, 80), (1, 1030, 33), (2, 513, 129), (1, 4100, 64)], ids=str)
+@pytest.mark.parametrize("B,T,C", [(1, 1, 1), (2, 1, 256), (3, 7, 5), (16, 200, 256), (2, 257, 80), (1, 1030, 33), (2, 513, 129), (1, 4100, 64), (2, 9000, 20)], ids=str)
 @pytest.mark.parametrize("ragged", [False, True], ids=["whole", "ragged"])
 def test_recurrence(B, T, C, ragged, dt):
     from ophelia_amd import modules as M
