@@ -139,7 +139,7 @@ class OphSeqRecur(C.Structure):
 SEQ_F32, SEQ_BF16, SEQ_F16 = 0, 1, 2
 # every symbol declared in include/ophelia_seq.h
 SEQ_LIBPATH = os.path.join(LIBDIR, "libophelia_seq.so")
-SEQ_SOURCES = ["oph_seq.hip", "oph_attn.hip", "oph_attngrad.hip", "oph_embed.hip", "oph_recur.hip"]
+SEQ_SOURCES = ["oph_seq.hip", "oph_attn.hip", "oph_attnfew.hip", "oph_attn32.hip", "oph_attngrad.hip", "oph_embed.hip", "oph_recur.hip"]
 SEQ_HEADERS = ["oph_seq.h", "oph_attn.h"]
 SEQ_SIGNATURES = {
     "oph_seq_abi_version": (C.c_int, []),

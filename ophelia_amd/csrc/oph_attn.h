@@ -149,6 +149,9 @@ template <class T, int DP, int ROWS, int THREADS> struct Stage {
     }
 };
 
+// rows of a unit of attn_split, attn_few and attn16_forward, whose splits attn_join joins
+template <class T> constexpr int unit_rows() { return sizeof(T) == 4 ? 16 : 32; }
+
 // writes of this wave to LDS are visible to its own later reads by other lanes
 __device__ __forceinline__ void wave_lds_fence() {
     __builtin_amdgcn_fence(__ATOMIC_RELEASE, "wavefront");
@@ -157,6 +160,8 @@ __device__ __forceinline__ void wave_lds_fence() {
 }
 
 // ---- host side -----------------------------------------------------------------------------------------------------------------
+int attn16_launch(const AttnP& p, int64_t groups, int what, void* stream);      // oph_attn32.hip: 0 forward, 1 dq, 2 dk and dv
+int attn_few_forward(const AttnP& p, int dtype, int64_t groups, void* stream);     // oph_attnfew.hip: M <= 4
 int attn_check(const oph_seq_attn* a, bool gradient);
 AttnP attn_params(const oph_seq_attn* a);
 int64_t attn_forward_workspace(const oph_seq_attn* a);

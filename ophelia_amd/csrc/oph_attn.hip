@@ -152,12 +152,12 @@ __global__ __launch_bounds__(256) void attn_wide(const AttnP p) {
     }
 }
 
-// ---- few rows: a workgroup of 4 waves shares 32 rows, every wave takes every fourth tile of 32 keys of its split; keys go straight
-// to the matrix operand, values through a tile of the wave's own.  With nsplit > 1 the results of the splits meet in attn_join. ----
+// ---- some rows, 16 bits (fp32: attn16_forward): a workgroup of 4 waves shares 32 rows, every wave takes every fourth tile of 32 keys of its
+// split; keys go straight to the matrix operand, values through a tile of the wave's own, for the transposed read.  With nsplit > 1
+// the results of the splits meet in attn_join. ----
 template <class T, int DP>
 __global__ __launch_bounds__(256) void attn_split(const AttnP p) {
-    constexpr int TB = Tile<T, DP>::bytes(32);
-    constexpr int JOIN = 4 * 32 * 36 * 4;
+    constexpr int TB = Tile<T, DP>::bytes(32), JOIN = 4 * 32 * 36 * 4;
     __shared__ __attribute__((aligned(16))) char lds[4 * TB > JOIN ? 4 * TB : JOIN];
     __shared__ float ml[4][32][2];
     const int tid = threadIdx.x, lane = tid & 63, wave = tid >> 6, half = lane >> 5, col = lane & 31;
@@ -180,15 +180,15 @@ __global__ __launch_bounds__(256) void attn_split(const AttnP p) {
     for (int d = 0; d < DP / 32; ++d) O[d] = f32x16{};
     const T* k = (const T*)p.k + w.b * p.ks[0] + w.hk * p.ks[2];
     const T* v = (const T*)p.v + w.b * p.vs[0] + w.hk * p.vs[2];
-    char* tv = lds + wave * TB;
     for (int key0 = kbeg + wave * 32; key0 < kend; key0 += 128) {
         const uint64_t bits = key_bits(p, w, key0, kend, lane) & 0xffffffffull;
         if (!bits) continue;
-        Stage<T, DP, 32, 64> sv;
         frag_t<T> K[DP / 16];
         row_frags<T, DP>(K, k + (int64_t)min(key0 + col, kend - 1) * p.ks[1], p.D, true, half);
-        sv.load([&](int r) { return v + (int64_t)min(key0 + r, kend - 1) * p.vs[1]; }, p.D, lane);
         f32x16 S[1] = {f32x16{}};
+        char* tv = lds + wave * TB;
+        Stage<T, DP, 32, 64> sv;
+        sv.load([&](int r) { return v + (int64_t)min(key0 + r, kend - 1) * p.vs[1]; }, p.D, lane);
 #pragma unroll
         for (int s = 0; s < DP / 16; ++s) S[0] = El<T>::mma(K[s], Q[s], S[0]);
         const float shrink = soft_step<1>(S, bits, st, c, half);
@@ -256,39 +256,53 @@ __global__ __launch_bounds__(256) void attn_split(const AttnP p) {
     }
 }
 
-// one wave per row: the splits' results, weighted to the common maximum, in the order of the splits (at most 64 of them)
+// a workgroup per row: the splits' results (at most 256), weighted to their common maximum; DP/4 threads hold the columns of a split,
+// the groups of threads take the splits in turn and are summed in their order
 template <class T, int DP>
 __global__ __launch_bounds__(256) void attn_join(const AttnP p) {
-    const int lane = threadIdx.x & 63, M = p.Tq * p.G, tiles = (M + 31) / 32;
-    const int64_t row = (int64_t)blockIdx.x * 4 + (threadIdx.x >> 6);
-    if (row >= (int64_t)p.B * p.Hk * M) return;
-    const int bh = (int)(row / M), r = (int)(row - (int64_t)bh * M);
+    constexpr int COLS = DP / 4, GROUPS = 256 / COLS;
+    __shared__ float weight[256];
+    __shared__ f32x4 sums[GROUPS][COLS];
+    const int tid = threadIdx.x, lane = tid & 63, M = p.Tq * p.G, RT = unit_rows<T>(), tiles = (M + RT - 1) / RT;
+    const int bh = blockIdx.x / M, r = blockIdx.x - bh * M;
     const int b = bh / p.Hk, hk = bh - b * p.Hk, t = row_time(p, r), h = hk * p.G + r - t * p.G;
     const int qlen = p.q_lens ? clampi(p.q_lens[b], 0, p.Tq) : p.Tq;
-    const int64_t unit = ((int64_t)bh * tiles + r / 32) * p.nsplit;
-    float m = -INFINITY, l = 0.f;
-    if (lane < p.nsplit) {
-        const float* at = p.aux + ((unit + lane) * 32 + r % 32) * 2;
-        m = at[0];
-        l = at[1];
-    }
-    float all = m;
+    const int64_t unit = ((int64_t)bh * tiles + r / RT) * p.nsplit;
+    float m[4], l[4], top = -INFINITY;                                     // every wave for itself: splits lane, lane + 64, ...
 #pragma unroll
-    for (int i = 32; i; i >>= 1) all = fmaxf(all, __shfl_xor(all, i));
-    const float weight = exp2_(m - (all == -INFINITY ? 0.f : all));
-    float sum = l * weight;
+    for (int i = 0; i < 4; ++i) {
+        const int s = lane + 64 * i;
+        const float* at = p.aux + ((unit + min(s, p.nsplit - 1)) * RT + r % RT) * 2;
+        m[i] = s < p.nsplit ? at[0] : -INFINITY;
+        l[i] = s < p.nsplit ? at[1] : 0.f;
+        top = fmaxf(top, m[i]);
+    }
+#pragma unroll
+    for (int i = 32; i; i >>= 1) top = fmaxf(top, __shfl_xor(top, i));
+    float sum = 0.f;
+#pragma unroll
+    for (int i = 0; i < 4; ++i) {
+        const float f = exp2_(m[i] - (top == -INFINITY ? 0.f : top));
+        sum += l[i] * f;
+        if (tid < 64) weight[lane + 64 * i] = f;
+    }
 #pragma unroll
     for (int i = 32; i; i >>= 1) sum += __shfl_xor(sum, i);
-    const int d = lane * 4;
+    __syncthreads();
+    const int g = tid / COLS, d = tid % COLS * 4;
     f32x4 o = {0.f, 0.f, 0.f, 0.f};
-    for (int s = 0; s < p.nsplit; ++s) {
-        const float ws = __shfl(weight, s);
-        if (d < p.D) o += *(const f32x4*)(p.part + ((unit + s) * 32 + r % 32) * DP + d) * ws;
-    }
+#pragma unroll 4
+    for (int s = g; s < p.nsplit; s += GROUPS)
+        if (d < p.D) o += *(const f32x4*)(p.part + ((unit + s) * RT + r % RT) * DP + d) * weight[s];
+    sums[g][tid % COLS] = o;
+    __syncthreads();
+    if (g) return;
+#pragma unroll
+    for (int i = 1; i < GROUPS; ++i) o += sums[i][tid];
     const bool live = t < qlen && sum != 0.f;
     const float inv = live ? 1.f / sum : 0.f;
     if (d < p.D) store4<T>((T*)p.o0 + (((int64_t)b * p.Tq + t) * (p.Hk * p.G) + h) * p.D + d, live ? o * inv : f32x4{0.f, 0.f, 0.f, 0.f});
-    if (lane == 0) p.lse[((int64_t)b * (p.Hk * p.G) + h) * p.Tq + t] = live ? (all + log2f(sum)) * LN2 : -INFINITY;
+    if (tid == 0) p.lse[((int64_t)b * (p.Hk * p.G) + h) * p.Tq + t] = live ? (top + log2f(sum)) * LN2 : -INFINITY;
 }
 
 // ---- host side --------------------------------------------------------------------------------------------------------------------
@@ -322,21 +336,28 @@ AttnP attn_params(const oph_seq_attn* a) {
 
 static int pad_d(int D) { return D <= 64 ? 64 : D <= 128 ? 128 : 256; }
 
-struct FwdPlan { bool wide; int nsplit; int64_t units; };
+struct FwdPlan { bool few, wide; int nsplit, rows; int64_t units; };
 static FwdPlan forward_plan(const oph_seq_attn* a) {
     const int64_t M = (int64_t)a->Tq * (a->Hq / a->Hk), heads = (int64_t)a->B * a->Hk;
     FwdPlan f;
-    f.wide = cdiv(M, 128) * heads >= 256;
-    f.units = cdiv(M, 32) * heads;
-    const int64_t fill = cdiv(512, f.units > 0 ? f.units : 1), most = cdiv(a->Tk, 128);
+    // without matrix instructions: 16 x 1 row over 150 keys x 256 fp32 7.7 us (29 on 32-row products), 8 x 8 heads x 4 rows over 1000 keys x 128
+    // bf16 15.0 (18.9); 4 rows of D <= 64 lose (8 x 8 heads over 4000 keys 25.7 and 20.6), 4 rows of D > 128 do not fit the registers
+    f.few = M <= 2 || (M <= 4 && a->D > 64 && a->D <= 128);
+    // 128-row workgroups once they fill the CUs (fp32, 4 x 8 heads of 1024 x 1024 x 128: 163 us, 16-row units 240); below, units that
+    // split the keys (16 sequences of 200 x 150 x 256: 21 and 63)
+    f.wide = !f.few && cdiv(M, 128) * heads >= 256;
+    f.rows = a->dtype == OPH_SEQ_F32 ? unit_rows<float>() : unit_rows<f16_t>();
+    f.units = cdiv(M, f.rows) * heads;
+    // one round of workgroups (two a CU; fp32 with D > 128 holds one a CU): a second, partly filled one costs more than longer loops
+    const int64_t fill = (a->dtype == OPH_SEQ_F32 && a->D > 128 ? 256 : 512) / (f.units > 0 ? f.units : 1), most = cdiv(a->Tk, f.few ? 256 : 128);
     const int64_t n = fill < most ? fill : most;
-    f.nsplit = f.wide ? 1 : (int)(n < 1 ? 1 : n > 64 ? 64 : n);
+    f.nsplit = f.wide ? 1 : (int)(n < 1 ? 1 : n > 256 ? 256 : n);
     return f;
 }
 
 int64_t attn_forward_workspace(const oph_seq_attn* a) {
     const FwdPlan f = forward_plan(a);
-    return f.nsplit == 1 ? 0 : f.units * f.nsplit * 32 * (pad_d(a->D) + 2) * (int64_t)sizeof(float);
+    return f.nsplit == 1 ? 0 : f.units * f.nsplit * f.rows * (pad_d(a->D) + 2) * (int64_t)sizeof(float);
 }
 
 template <class T, int DP, int KT, int NQ> static int forward(const oph_seq_attn* a, const FwdPlan& f, AttnP& p, void* stream) {
@@ -344,9 +365,14 @@ template <class T, int DP, int KT, int NQ> static int forward(const oph_seq_attn
     if (f.wide) return launch<AttnP>(attn_wide<T, DP, KT, NQ>, dim3((unsigned)(cdiv(M, 128 * NQ) * heads)), 256, p, 0, stream);
     p.nsplit = f.nsplit;
     p.part = (float*)a->workspace;
-    p.aux = p.part + f.units * f.nsplit * 32 * DP;
-    if (int rc = launch<AttnP>(attn_split<T, DP>, dim3((unsigned)(f.units * f.nsplit)), 256, p, 0, stream)) return rc;
-    if (f.nsplit > 1) return launch<AttnP>(attn_join<T, DP>, dim3((unsigned)cdiv(M * heads, 4)), 256, p, 0, stream);
+    p.aux = p.part + f.units * f.nsplit * f.rows * DP;
+    const int64_t groups = f.units * f.nsplit;
+    int rc;
+    if (f.few) rc = attn_few_forward(p, a->dtype, groups, stream);
+    else if constexpr (sizeof(T) == 4) rc = attn16_launch(p, groups, 0, stream);
+    else rc = launch<AttnP>(attn_split<T, DP>, dim3((unsigned)groups), 256, p, 0, stream);
+    if (rc) return rc;
+    if (f.nsplit > 1) return launch<AttnP>(attn_join<T, DP>, dim3((unsigned)(M * heads)), 256, p, 0, stream);
     return OPH_OK;
 }
 template <class T> static int forward_d(const oph_seq_attn* a, const FwdPlan& f, AttnP& p, void* stream) {

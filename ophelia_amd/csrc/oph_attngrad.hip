@@ -261,20 +261,24 @@ template <class T> __global__ __launch_bounds__(256) void attn_sum(const SumP p)
 }
 
 // ---- host side -------------------------------------------------------------------------------------------------------------------------
-struct GradPlan { int dq_split, kv_split; int64_t dq_units, kv_units, nq, nk; bool both; };
-static int split_for(int64_t groups, int64_t pieces) {
-    const int64_t n = groups > 0 ? cdiv(512, groups) : 1;
-    const int64_t k = n < pieces ? n : pieces;
+struct GradPlan { bool small; int dq_split, kv_split; int64_t dq_units, kv_units, nq, nk; };
+static int split_for(int64_t units, int64_t pieces, int64_t groups) {
+    const int64_t n = units > 0 ? groups / units : 1, k = n < pieces ? n : pieces;
     return (int)(k < 1 ? 1 : k > 16 ? 16 : k);
 }
 static GradPlan gradient_plan(const oph_seq_attn* a) {
     const int64_t M = (int64_t)a->Tq * (a->Hq / a->Hk), heads = (int64_t)a->B * a->Hk;
     GradPlan g;
-    g.both = a->D <= 128;
-    g.dq_units = cdiv(M, 128) * heads;
-    g.kv_units = cdiv(a->Tk, 128) * heads * (g.both ? 1 : 2);
-    g.dq_split = split_for(g.dq_units, cdiv(a->Tk, 128));
-    g.kv_split = split_for(g.kv_units, cdiv(M, 128));
+    // fp32 on 16x16 products: where 128 x 128 tiles are too few to fill the machine (16 sequences of 200 x 150 x 256: 75 us, 231 on the large
+    // tiles; 4 x 4 heads of 100 x 1500 x 64: 54 and 62), and for D > 128, where the large tiles' operands do not fit the registers (4 x 8 heads
+    // of 1024 x 1024 x 256: 2480 and 2817).  Elsewhere the shared tiles win (4 x 8 heads of 2048 x 256 x 64: 151 and 242).
+    g.small = a->dtype == OPH_SEQ_F32 && (a->D > 128 || cdiv(M, 128) * heads * cdiv(a->Tk, 128) * (a->D <= 64 ? 64 : 128) < 16384);
+    const int rows = g.small ? 16 : 128, keys = g.small ? 16 : 128;
+    g.dq_units = cdiv(M, rows) * heads;
+    g.kv_units = cdiv(a->Tk, keys) * heads * (g.small || a->D <= 128 ? 1 : 2);
+    const int64_t groups = a->D > 128 ? 256 : 512;                          // one round: one or two workgroups a CU
+    g.dq_split = split_for(g.dq_units, cdiv(a->Tk, 128), groups);
+    g.kv_split = split_for(g.kv_units, cdiv(M, 128), groups);
     g.nq = (int64_t)a->B * a->Tq * a->Hq * a->D;
     g.nk = (int64_t)a->B * a->Tk * a->Hk * a->D;
     return g;
@@ -295,7 +299,11 @@ template <class T, int DP> static int gradient(const oph_seq_attn* a, AttnP p, v
     if (g.nq) {
         p.nsplit = g.dq_split;
         p.o0 = a->dq;
-        if (int rc = launch<AttnP>(attn_dq<T, DP>, dim3((unsigned)(g.dq_units * g.dq_split)), 256, p, 0, stream)) return rc;
+        const int64_t groups = g.dq_units * g.dq_split;
+        int rc;
+        if constexpr (sizeof(T) == 4 && DP > 128) rc = attn16_launch(p, groups, 1, stream);
+        else rc = g.small ? attn16_launch(p, groups, 1, stream) : launch<AttnP>(attn_dq<T, DP>, dim3((unsigned)groups), 256, p, 0, stream);
+        if (rc) return rc;
         if (g.dq_split > 1) {
             if (int rc = sum<T>(p.part, a->dq, nullptr, g.nq, g.dq_split, stream)) return rc;
         }
@@ -304,7 +312,11 @@ template <class T, int DP> static int gradient(const oph_seq_attn* a, AttnP p, v
         p.nsplit = g.kv_split;
         p.o0 = a->dv;
         p.o1 = a->dk;
-        if (int rc = launch<AttnP>(attn_dkv<T, DP, DP <= 128>, dim3((unsigned)(g.kv_units * g.kv_split)), 256, p, 0, stream)) return rc;
+        const int64_t groups = g.kv_units * g.kv_split;
+        int rc;
+        if constexpr (sizeof(T) == 4 && DP > 128) rc = attn16_launch(p, groups, 2, stream);
+        else rc = g.small ? attn16_launch(p, groups, 2, stream) : launch<AttnP>(attn_dkv<T, DP, DP <= 128>, dim3((unsigned)groups), 256, p, 0, stream);
+        if (rc) return rc;
         if (g.kv_split > 1) return sum<T>(p.part, a->dv, a->dk, g.nk, g.kv_split, stream);
     }
     return OPH_OK;
