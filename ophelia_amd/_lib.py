@@ -268,6 +268,12 @@ def load_seq():
         raise OpheliaHipError(
             "HIP extension %s is missing: run `python -c 'import __graft_entry__ as g; g.build()'` "
             "(there is no CPU fallback)" % SEQ_LIBPATH)
+    # The tensors and streams are torch's, and torch may bring a HIP runtime of its own beside the one that libophelia_hip.so has loaded
+    # (it asks for it by another name): that one goes to the front of the symbol search, so that both work with the same streams.
+    import torch
+    runtime = os.path.join(os.path.dirname(torch.__file__), "lib", "libamdhip64.so")
+    if os.path.exists(runtime):
+        C.CDLL(runtime, mode=C.RTLD_GLOBAL)
     lib = C.CDLL(SEQ_LIBPATH)
     for name, (res, args) in SEQ_SIGNATURES.items():
         fn = getattr(lib, name)

@@ -84,10 +84,11 @@ __device__ __forceinline__ void row_frags(frag_t<T> (&f)[DP / 16], const T* row,
     }
 }
 
-// A tile of rows in LDS, row-major.  32 bytes of padding: the rows' 16-byte pieces fall on 8 different bank groups for reads along a
-// row, and 4 rows x 32 bytes (16 bit) or 2 x 128 bytes (fp32) of a transposed read are 64 different banks.
+// A tile of rows in LDS, row-major.  The padding spreads the rows' pieces over the banks, for reads along a row (16 bytes of 32 rows)
+// and across (4 rows x 32 bytes, or 2 x 128): of 16, 32, 48 and 64 bytes 48 leaves the fewest conflicts (a third of 16's and 64's; 4 x 16 heads
+// of 4096 x 4096 x 128 bf16: 610, 577, 571 and 605 us).
 template <class T, int DP> struct Tile {
-    static constexpr int STRIDE = DP * (int)sizeof(T) + 32;
+    static constexpr int STRIDE = DP * (int)sizeof(T) + 48;
     static constexpr int bytes(int rows) { return rows * STRIDE; }
 };
 
@@ -129,23 +130,35 @@ template <class T> __device__ __forceinline__ frag_t<T> next_frag(const f32x16& 
 
 // Rows on their way from memory to a tile: load() issues the loads, store() writes what is valid and zeros elsewhere.
 template <class T, int DP, int ROWS, int THREADS> struct Stage {
-    static constexpr int PER = El<T>::PER16, CPR = DP / PER, N = ROWS * CPR / THREADS;
-    static_assert(ROWS * CPR % THREADS == 0 && (THREADS % CPR == 0 || CPR % THREADS == 0), "Stage");
+    static constexpr int PER = El<T>::PER16, CPR = DP / PER, N = ROWS * CPR / THREADS, STEP = THREADS / CPR;
+    static_assert(ROWS * CPR % THREADS == 0 && THREADS % CPR == 0, "Stage");
     u32x4 x[N];
     template <class F> __device__ __forceinline__ void load(F row, int D, int tid) {
+        const int d = tid % CPR * PER;
 #pragma unroll
-        for (int i = 0; i < N; ++i) {
-            const int c = i * THREADS + tid, r = c / CPR, d = (c % CPR) * PER;
-            x[i] = load16(row(r) + (d < D ? d : 0));
-        }
+        for (int i = 0; i < N; ++i) x[i] = load16(row(i * STEP + tid / CPR) + (d < D ? d : 0));
+    }
+    // consecutive rows that are all there: `at` is this thread's place in the first of them (own()), no multiplications on the way
+    static __device__ __forceinline__ const T* own(const T* first, int64_t stride, int D, int tid) {
+        const int d = tid % CPR * PER;
+        return first + tid / CPR * stride + (d < D ? d : 0);
+    }
+    __device__ __forceinline__ void load_run(const T* at, int64_t stride) {
+#pragma unroll
+        for (int i = 0; i < N; ++i) x[i] = load16(at + i * (STEP * stride));
     }
     __device__ __forceinline__ void store(char* tile, uint64_t bits, int D, int tid) const {
+        constexpr uint64_t FULL = ROWS == 64 ? ~0ull : (1ull << (ROWS & 63)) - 1;
+        char* at = tile + tid / CPR * Tile<T, DP>::STRIDE + tid % CPR * 16;
+        if (bits == FULL && D == DP) {
 #pragma unroll
-        for (int i = 0; i < N; ++i) {
-            const int c = i * THREADS + tid, r = c / CPR, d = (c % CPR) * PER;
-            const bool ok = ((bits >> r) & 1) && d < D;
-            *(u32x4*)(tile + r * Tile<T, DP>::STRIDE + d * (int)sizeof(T)) = ok ? x[i] : u32x4{0, 0, 0, 0};
+            for (int i = 0; i < N; ++i) *(u32x4*)(at + i * (STEP * Tile<T, DP>::STRIDE)) = x[i];
+            return;
         }
+        const bool in = tid % CPR * PER < D;
+#pragma unroll
+        for (int i = 0; i < N; ++i)
+            *(u32x4*)(at + i * (STEP * Tile<T, DP>::STRIDE)) = in && ((bits >> (i * STEP + tid / CPR)) & 1) ? x[i] : u32x4{0, 0, 0, 0};
     }
 };
 

@@ -26,7 +26,9 @@ template <int N> __device__ __forceinline__ float soft_step(f32x16 (&S)[N], uint
 #pragma unroll
         for (int r = 0; r < 16; ++r) mx = fmaxf(mx, S[n][r]);
     mx = fmaxf(mx, other_half(mx));
-    const float m = fmaxf(st.m, mx * c);
+    // The reference point moves only when a score passes it by more than 2^8: probabilities stay below 256 (their relative precision is
+    // the same), and results are rescaled a few times a row instead of at every new maximum.
+    const float m = mx * c > st.m + 8.f ? mx * c : st.m;
     const float base = m == -INFINITY ? 0.f : m;       // a row without a finite score so far: every exponential below is 0
     const float shrink = exp2_(st.m - base);
     float sum = 0.f;
@@ -43,8 +45,11 @@ template <int N> __device__ __forceinline__ float soft_step(f32x16 (&S)[N], uint
 }
 
 // ---- many rows: a workgroup of 4 waves, 32*NQ rows each, over all keys; key and value tiles in LDS for the four -----------------------
+// waves a SIMD that the registers must leave room for: a second wave's products run under the first one's exponentials (4 x 16 heads
+// of 4096 x 4096 x 128: 576 us with two waves, 970 with one; D = 64: three)
+template <class T, int DP> constexpr int wide_waves() { return sizeof(T) == 4 || DP > 128 ? 1 : DP > 64 ? 2 : 3; }
 template <class T, int DP, int KT, int NQ>
-__global__ __launch_bounds__(256) void attn_wide(const AttnP p) {
+__global__ __launch_bounds__(256, (wide_waves<T, DP>())) void attn_wide(const AttnP p) {
     constexpr int ROWS = 128 * NQ, NK = KT / 32, TB = Tile<T, DP>::bytes(KT);
     __shared__ __attribute__((aligned(16))) char lds[4 * TB];
     const int tid = threadIdx.x, lane = tid & 63, wave = tid >> 6, half = lane >> 5, col = lane & 31;
@@ -70,10 +75,18 @@ __global__ __launch_bounds__(256) void attn_wide(const AttnP p) {
     const bool any = row_time(p, w.tile * ROWS) < w.qlen;               // a tile of padding only: nothing to read
     const int nt = any ? (w.klen + KT - 1) / KT : 0;
     Stage<T, DP, KT, 256> sk, sv;
+    const T *k1 = sk.own(k, p.ks[1], p.D, tid), *v1 = sv.own(v, p.vs[1], p.D, tid);
     uint64_t bits = 0, next = 0;
     auto fetch = [&](int j) {
         const int key0 = j * KT, last = w.klen - 1;
         next = key_bits(p, w, key0, w.klen, lane) & (KT == 64 ? ~0ull : 0xffffffffull);
+        if (key0 + KT <= w.klen) {
+            sk.load_run(k1, p.ks[1]);
+            sv.load_run(v1, p.vs[1]);
+            k1 += KT * p.ks[1];
+            v1 += KT * p.vs[1];
+            return;
+        }
         sk.load([&](int r) { return k + (int64_t)min(key0 + r, last) * p.ks[1]; }, p.D, tid);
         sv.load([&](int r) { return v + (int64_t)min(key0 + r, last) * p.vs[1]; }, p.D, tid);
     };

@@ -18,9 +18,14 @@ __device__ __forceinline__ float dot8(f32x8 a, f32x8 b) {
 }
 
 // ---- dq: S^T = K q^T and dP^T = V dout^T have the queries as columns; dS^T is the operand of dq^T = K^T dS^T -------------------------------
+// 16 bits: waves a SIMD that the registers must leave room for, and rows of a tile in LDS -- D = 64 has few products between two barriers
+// (2 x 16 heads of 4096 x 4096 x 64: 499 us, with tiles of 32 rows 608).
+template <class T, int DP> constexpr int grad_waves(int of64) { return sizeof(T) == 4 || DP > 128 ? 1 : DP > 64 ? 2 : of64; }
+template <class T, int DP> constexpr int grad_tile() { return sizeof(T) == 2 && DP == 64 ? 64 : 32; }
 template <class T, int DP>
-__global__ __launch_bounds__(256) void attn_dq(const AttnP p) {
-    constexpr int KT = 32, TB = Tile<T, DP>::bytes(KT);
+__global__ __launch_bounds__(256, (grad_waves<T, DP>(3))) void attn_dq(const AttnP p) {
+    constexpr int KT = grad_tile<T, DP>(), TB = Tile<T, DP>::bytes(KT);
+    constexpr uint64_t FULL = KT == 64 ? ~0ull : 0xffffffffull;
     __shared__ __attribute__((aligned(16))) char lds[4 * TB];
     const int tid = threadIdx.x, lane = tid & 63, wave = tid >> 6, half = lane >> 5, col = lane & 31;
     const int M = p.Tq * p.G, Hq = p.Hk * p.G, tiles = (M + 127) / 128;
@@ -62,10 +67,18 @@ __global__ __launch_bounds__(256) void attn_dq(const AttnP p) {
     const int kbeg = split * per, kend = row_time(p, w.tile * 128) < w.qlen ? min(w.klen, kbeg + per) : kbeg;
     const int nt = kend > kbeg ? (kend - kbeg + KT - 1) / KT : 0;
     Stage<T, DP, KT, 256> sk, sv;
+    const T *k1 = sk.own(k + kbeg * p.ks[1], p.ks[1], p.D, tid), *v1 = sv.own(v + kbeg * p.vs[1], p.vs[1], p.D, tid);
     uint64_t bits = 0, next = 0;
     auto fetch = [&](int j) {
         const int key0 = kbeg + j * KT, last = kend - 1;
-        next = key_bits(p, w, key0, kend, lane) & 0xffffffffull;
+        next = key_bits(p, w, key0, kend, lane) & FULL;
+        if (key0 + KT <= kend) {
+            sk.load_run(k1, p.ks[1]);
+            sv.load_run(v1, p.vs[1]);
+            k1 += KT * p.ks[1];
+            v1 += KT * p.vs[1];
+            return;
+        }
         sk.load([&](int i) { return k + (int64_t)min(key0 + i, last) * p.ks[1]; }, p.D, tid);
         sv.load([&](int i) { return v + (int64_t)min(key0 + i, last) * p.vs[1]; }, p.D, tid);
     };
@@ -82,23 +95,27 @@ __global__ __launch_bounds__(256) void attn_dq(const AttnP p) {
         if (j + 1 < nt) fetch(j + 1);
         if (now) {
             const char *tk = lds + (j & 1) * 2 * TB, *tv = tk + TB;
-            f32x16 S = {}, dP = {};
 #pragma unroll
-            for (int s = 0; s < DP / 16; ++s) {
-                S = El<T>::mma(row_frag<T, DP>(tk, 0, s, lane), Q[s], S);
-                dP = El<T>::mma(row_frag<T, DP>(tv, 0, s, lane), dO[s], dP);
-            }
-            const uint32_t b = (uint32_t)now >> (4 * half);
+            for (int k0 = 0; k0 < KT; k0 += 32) {
+                f32x16 S = {}, dP = {};
 #pragma unroll
-            for (int i = 0; i < 16; ++i) {
-                const float x = exp2_(fmaf(S[i], c, -lse2)) * (dP[i] - delta);
-                S[i] = now == 0xffffffffull || ((b >> (8 * (i / 4) + i % 4)) & 1) ? x : 0.f;
-            }
+                for (int s = 0; s < DP / 16; ++s) {
+                    S = El<T>::mma(row_frag<T, DP>(tk, k0, s, lane), Q[s], S);
+                    dP = El<T>::mma(row_frag<T, DP>(tv, k0, s, lane), dO[s], dP);
+                }
+                const uint32_t b = (uint32_t)(now >> k0) >> (4 * half);
 #pragma unroll
-            for (int s = 0; s < 2; ++s) {
-                const frag_t<T> dS = next_frag<T>(S, s);
+                for (int i = 0; i < 16; ++i) S[i] = exp2_(fmaf(S[i], c, -lse2)) * (dP[i] - delta);
+                if (now != FULL) {
 #pragma unroll
-                for (int d = 0; d < DP / 32; ++d) dQ[d] = El<T>::mma(trans_frag<T, DP>(tk, 16 * s, 32 * d, lane), dS, dQ[d]);
+                    for (int i = 0; i < 16; ++i) S[i] = (b >> (8 * (i / 4) + i % 4)) & 1 ? S[i] : 0.f;
+                }
+#pragma unroll
+                for (int s = 0; s < 2; ++s) {
+                    const frag_t<T> dS = next_frag<T>(S, s);
+#pragma unroll
+                    for (int d = 0; d < DP / 32; ++d) dQ[d] = El<T>::mma(trans_frag<T, DP>(tk, k0 + 16 * s, 32 * d, lane), dS, dQ[d]);
+                }
             }
         }
         if (j + 1 < nt) commit(j + 1);
@@ -127,9 +144,12 @@ __global__ __launch_bounds__(256) void attn_dq(const AttnP p) {
 // BOTH: one workgroup forms both.  Otherwise (D > 128: both results and both key operands do not fit the registers) half of the grid
 // forms dv and half dk, and the scores are formed twice. ----
 template <class T, int DP, bool BOTH>
-__global__ __launch_bounds__(256) void attn_dkv(const AttnP p) {
-    constexpr int RT = 32, TB = Tile<T, DP>::bytes(RT), NACC = BOTH ? 2 : 1;
-    __shared__ __attribute__((aligned(16))) char lds[4 * TB];
+__global__ __launch_bounds__(256, (grad_waves<T, DP>(2))) void attn_dkv(const AttnP p) {
+    constexpr int RT = grad_tile<T, DP>(), TB = Tile<T, DP>::bytes(RT), TV = Tile<T, DP>::bytes(32), NACC = BOTH ? 2 : 1;
+    // 16 bits, D = 128: with the values' operand in LDS too the rest fits the 256 registers that two waves a SIMD leave each (in registers, 21
+    // words were spilled, prefetched tiles among them: 1115 us for both passes over 2 x 16 heads of 4096 x 4096 instead of 1005)
+    constexpr bool VLDS = sizeof(T) == 2 && DP == 128;
+    __shared__ __attribute__((aligned(16))) char lds[4 * TB + (VLDS ? 4 * TV : 0)];
     __shared__ __attribute__((aligned(16))) float stat[2][2][RT];       // lse (units of log2) and delta of a tile's rows
     const int tid = threadIdx.x, lane = tid & 63, wave = tid >> 6, half = lane >> 5, col = lane & 31;
     const int Hq = p.Hk * p.G, tiles = (p.Tk + 127) / 128;
@@ -146,7 +166,15 @@ __global__ __launch_bounds__(256) void attn_dkv(const AttnP p) {
     f32x16 acc[NACC][DP / 32];                                            // dv first
     const int64_t kk = min(key, p.Tk - 1);
     row_frags<T, DP>(K, (const T*)p.k + w.b * p.ks[0] + w.hk * p.ks[2] + kk * p.ks[1], p.D, ok, half);
-    if (BOTH || want_dk) row_frags<T, DP>(V, (const T*)p.v + w.b * p.vs[0] + w.hk * p.vs[2] + kk * p.vs[1], p.D, ok, half);
+    char* tv = lds + 4 * TB + wave * TV;
+    if (BOTH || want_dk) {
+        row_frags<T, DP>(V, (const T*)p.v + w.b * p.vs[0] + w.hk * p.vs[2] + kk * p.vs[1], p.D, ok, half);
+        if constexpr (VLDS) {
+#pragma unroll
+            for (int s = 0; s < DP / 16; ++s) *(frag_t<T>*)(tv + col * Tile<T, DP>::STRIDE + (s * 16 + half * 8) * 2) = V[s];
+            wave_lds_fence();
+        }
+    }
 #pragma unroll
     for (int a = 0; a < NACC; ++a)
 #pragma unroll
@@ -158,10 +186,26 @@ __global__ __launch_bounds__(256) void attn_dkv(const AttnP p) {
     const int nt = rend > rbeg ? (rend - rbeg + RT - 1) / RT : 0;
     Stage<T, DP, RT, 256> sq, so;
     float lse2 = INFINITY, delta = 0.f;
+    // where the group divides the rows that a thread's pieces lie apart, those and the next tile's are the same heads at later steps
+    const bool even = sq.STEP % p.G == 0;
+    const int64_t qstep = sq.STEP / p.G * p.qs[1], ostep = sq.STEP / p.G * p.ds[1];
+    const int r1 = rbeg + tid / sq.CPR, d1 = tid % sq.CPR * sq.PER < p.D ? tid % sq.CPR * sq.PER : 0;
+    const T* q1 = row_ptr<T>(p, p.q, w, r1, p.qs[0], p.qs[1], p.qs[2]) + d1;
+    const T* o1 = row_ptr<T>(p, p.dout, w, r1, p.ds[0], p.ds[1], p.ds[2]) + d1;
     auto fetch = [&](int j) {
         const int r0 = rbeg + j * RT;
-        sq.load([&](int i) { return row_ptr<T>(p, p.q, w, r0 + i, p.qs[0], p.qs[1], p.qs[2]); }, p.D, tid);
-        so.load([&](int i) { return row_ptr<T>(p, p.dout, w, r0 + i, p.ds[0], p.ds[1], p.ds[2]); }, p.D, tid);
+        if (even && r0 + RT <= rend) {
+#pragma unroll
+            for (int i = 0; i < sq.N; ++i) {
+                sq.x[i] = load16(q1);
+                so.x[i] = load16(o1);
+                q1 += qstep;
+                o1 += ostep;
+            }
+        } else {
+            sq.load([&](int i) { return row_ptr<T>(p, p.q, w, r0 + i, p.qs[0], p.qs[1], p.qs[2]); }, p.D, tid);
+            so.load([&](int i) { return row_ptr<T>(p, p.dout, w, r0 + i, p.ds[0], p.ds[1], p.ds[2]); }, p.D, tid);
+        }
         if (tid < RT) {
             const int r = r0 + tid, t = row_time(p, r);
             lse2 = INFINITY;
@@ -177,7 +221,7 @@ __global__ __launch_bounds__(256) void attn_dkv(const AttnP p) {
     auto commit = [&](int j) {
         char* x = lds + (j & 1) * 2 * TB;
         const int left = rend - (rbeg + j * RT);
-        const uint64_t bits = left >= RT ? 0xffffffffull : (1ull << left) - 1;
+        const uint64_t bits = left >= RT ? (RT == 64 ? ~0ull : 0xffffffffull) : (1ull << left) - 1;
         sq.store(x, bits, p.D, tid);
         so.store(x + TB, bits, p.D, tid);
         if (tid < RT) { stat[j & 1][0][tid] = lse2; stat[j & 1][1][tid] = delta; }
@@ -187,39 +231,42 @@ __global__ __launch_bounds__(256) void attn_dkv(const AttnP p) {
         __syncthreads();
         if (j + 1 < nt) fetch(j + 1);
         const char *tq = lds + (j & 1) * 2 * TB, *to = tq + TB;
-        f32x16 S = {};
 #pragma unroll
-        for (int s = 0; s < DP / 16; ++s) S = El<T>::mma(row_frag<T, DP>(tq, 0, s, lane), K[s], S);
+        for (int q0 = 0; q0 < RT; q0 += 32) {
+            f32x16 S = {};
 #pragma unroll
-        for (int g = 0; g < 4; ++g) {
-            const f32x4 l = *(const f32x4*)&stat[j & 1][0][8 * g + 4 * half];
-#pragma unroll
-            for (int i = 0; i < 4; ++i) S[4 * g + i] = exp2_(fmaf(S[4 * g + i], c, -l[i]));
-        }
-        if (BOTH || !want_dk) {
-#pragma unroll
-            for (int s = 0; s < 2; ++s) {
-                const frag_t<T> P = next_frag<T>(S, s);
-#pragma unroll
-                for (int d = 0; d < DP / 32; ++d) acc[0][d] = El<T>::mma(trans_frag<T, DP>(to, 16 * s, 32 * d, lane), P, acc[0][d]);
-            }
-        }
-        if (BOTH || want_dk) {
-            f32x16 dP = {};
-#pragma unroll
-            for (int s = 0; s < DP / 16; ++s) dP = El<T>::mma(row_frag<T, DP>(to, 0, s, lane), V[s], dP);
+            for (int s = 0; s < DP / 16; ++s) S = El<T>::mma(row_frag<T, DP>(tq, q0, s, lane), K[s], S);
 #pragma unroll
             for (int g = 0; g < 4; ++g) {
-                const f32x4 x = *(const f32x4*)&stat[j & 1][1][8 * g + 4 * half];
+                const f32x4 l = *(const f32x4*)&stat[j & 1][0][q0 + 8 * g + 4 * half];
 #pragma unroll
-                for (int i = 0; i < 4; ++i) S[4 * g + i] *= dP[4 * g + i] - x[i];
+                for (int i = 0; i < 4; ++i) S[4 * g + i] = exp2_(fmaf(S[4 * g + i], c, -l[i]));
             }
+            if (BOTH || !want_dk) {
 #pragma unroll
-            for (int s = 0; s < 2; ++s) {
-                const frag_t<T> dS = next_frag<T>(S, s);
+                for (int s = 0; s < 2; ++s) {
+                    const frag_t<T> P = next_frag<T>(S, s);
 #pragma unroll
-                for (int d = 0; d < DP / 32; ++d)
-                    acc[NACC - 1][d] = El<T>::mma(trans_frag<T, DP>(tq, 16 * s, 32 * d, lane), dS, acc[NACC - 1][d]);
+                    for (int d = 0; d < DP / 32; ++d) acc[0][d] = El<T>::mma(trans_frag<T, DP>(to, q0 + 16 * s, 32 * d, lane), P, acc[0][d]);
+                }
+            }
+            if (BOTH || want_dk) {
+                f32x16 dP = {};
+#pragma unroll
+                for (int s = 0; s < DP / 16; ++s) dP = El<T>::mma(row_frag<T, DP>(to, q0, s, lane), VLDS ? row_frag<T, DP>(tv, 0, s, lane) : V[s], dP);
+#pragma unroll
+                for (int g = 0; g < 4; ++g) {
+                    const f32x4 x = *(const f32x4*)&stat[j & 1][1][q0 + 8 * g + 4 * half];
+#pragma unroll
+                    for (int i = 0; i < 4; ++i) S[4 * g + i] *= dP[4 * g + i] - x[i];
+                }
+#pragma unroll
+                for (int s = 0; s < 2; ++s) {
+                    const frag_t<T> dS = next_frag<T>(S, s);
+#pragma unroll
+                    for (int d = 0; d < DP / 32; ++d)
+                        acc[NACC - 1][d] = El<T>::mma(trans_frag<T, DP>(tq, q0 + 16 * s, 32 * d, lane), dS, acc[NACC - 1][d]);
+                }
             }
         }
         if (j + 1 < nt) commit(j + 1);

@@ -497,3 +497,17 @@ def test_refusals():
                  lambda: M.cross_attention(q, k, k, scale=-1.0), lambda: M.embed_lookup(lens, torch.zeros(4, 4, device="cuda"), scale=math.inf)):
         with pytest.raises(_lib.OpheliaHipError):
             call()
+
+
+def test_synthesis_library_loaded_before_torch():
+    """libophelia_hip.so loads the system's HIP runtime, torch may bring its own under another name: the operators must find torch's, also on
+    a stream of torch's."""
+    import subprocess
+    import sys
+    from conftest import ROOT
+    code = ("from ophelia_amd import _lib; _lib.load(); from ophelia_amd import modules as M; "
+            "import torch; s = torch.cuda.Stream(); t = torch.arange(12., device='cuda').view(4, 3); torch.cuda.synchronize();\n"
+            "with torch.cuda.stream(s): r = M.embed_lookup(torch.tensor([2, 1], device='cuda'), t)\n"
+            "s.synchronize(); assert r.tolist() == [[6., 7., 8.], [3., 4., 5.]], r; print('right')")
+    r = subprocess.run([sys.executable, "-c", code], cwd=ROOT, capture_output=True, text=True, timeout=100)
+    assert r.returncode == 0 and "right" in r.stdout, (r.returncode, r.stdout[-500:], r.stderr[-1500:])
