@@ -137,24 +137,24 @@ class OphSeqRecur(C.Structure):
 
 
 SEQ_F32, SEQ_BF16, SEQ_F16 = 0, 1, 2
-# every symbol declared in include/ophelia_seq.h
+# every symbol declared in include/ophelia_seq.h; argument structures go as a pointer to an OphSeq* or as their packed bytes
 SEQ_LIBPATH = os.path.join(LIBDIR, "libophelia_seq.so")
 SEQ_SOURCES = ["oph_seq.hip", "oph_attn.hip", "oph_attnfew.hip", "oph_attn32.hip", "oph_attngrad.hip", "oph_embed.hip", "oph_recur.hip"]
 SEQ_HEADERS = ["oph_seq.h", "oph_attn.h"]
 SEQ_SIGNATURES = {
     "oph_seq_abi_version": (C.c_int, []),
     "oph_seq_last_error": (C.c_char_p, []),
-    "oph_seq_attn_workspace": (C.c_int64, [C.POINTER(OphSeqAttn), C.c_int]),
-    "oph_seq_attn_forward": (C.c_int, [C.POINTER(OphSeqAttn), C.c_int, C.c_void_p]),
-    "oph_seq_attn_gradient": (C.c_int, [C.POINTER(OphSeqAttn), C.c_int, C.c_void_p]),
+    "oph_seq_attn_workspace": (C.c_int64, [C.c_void_p, C.c_int]),
+    "oph_seq_attn_forward": (C.c_int, [C.c_void_p, C.c_int, C.c_void_p]),
+    "oph_seq_attn_gradient": (C.c_int, [C.c_void_p, C.c_int, C.c_void_p]),
     "oph_seq_embed_lookup": (C.c_int, [C.c_void_p, C.c_int, C.c_int64, C.c_void_p, C.c_int64, C.c_int, C.c_int, C.c_float, C.c_int, C.c_int,
                                        C.c_void_p, C.c_int, C.c_void_p]),
     "oph_seq_embed_workspace": (C.c_int64, [C.c_int64, C.c_int, C.c_int]),
     "oph_seq_embed_gradient": (C.c_int, [C.c_void_p, C.c_int, C.c_int64, C.c_void_p, C.c_int64, C.c_int, C.c_int, C.c_float, C.c_int, C.c_int,
                                          C.c_void_p, C.c_void_p, C.c_size_t, C.c_int, C.c_void_p]),
-    "oph_seq_recur_workspace": (C.c_int64, [C.POINTER(OphSeqRecur), C.c_int]),
-    "oph_seq_recur_forward": (C.c_int, [C.POINTER(OphSeqRecur), C.c_int, C.c_void_p]),
-    "oph_seq_recur_gradient": (C.c_int, [C.POINTER(OphSeqRecur), C.c_int, C.c_void_p]),
+    "oph_seq_recur_workspace": (C.c_int64, [C.c_void_p, C.c_int]),
+    "oph_seq_recur_forward": (C.c_int, [C.c_void_p, C.c_int, C.c_void_p]),
+    "oph_seq_recur_gradient": (C.c_int, [C.c_void_p, C.c_int, C.c_void_p]),
 }
 
 _lib = None

@@ -11,18 +11,26 @@ synchronise, so they can be captured into a graph.  Sums, statistics and states 
 which workgroups run.  Gradients are functions of their own: nothing here records for torch's autograd, and tensors that
 require gradients are refused outside torch.no_grad().  Bad arguments raise ValueError before anything is queued; there is
 no CPU fallback."""
-import ctypes as C
-import math
+import struct
 
 from . import _lib
 
 _T = {}
+_state = {}
+# the argument structures of include/ophelia_seq.h as the compiler lays them out: packing them in one go is a third of the time that filling
+# ctypes fields takes, and a call on small tensors is bound by what happens here
+_ATTN = struct.Struct("@12P14qPN7if")
+_RECUR = struct.Struct("@11P8qPN4i")
+_NO_STRIDES = (0, 0, 0)
 
 
 def _torch():
     import torch
     if not _T:
         _T.update({torch.float32: _lib.SEQ_F32, torch.bfloat16: _lib.SEQ_BF16, torch.float16: _lib.SEQ_F16})
+        # the raw handle of the current stream without the stream object around it, where this torch has it
+        raw = getattr(torch._C, "_cuda_getCurrentRawStream", None)
+        _state["stream"] = raw or (lambda index: torch.cuda.current_stream(index).cuda_stream)
     return torch
 
 
@@ -32,57 +40,49 @@ def _chk(rc):
     return rc
 
 
-def _need(ok, text, *args):
-    if not ok:
-        raise ValueError(text % args)
-
-
 def _first(torch, name, t):
     """Checks the tensor that decides type and device of a call."""
-    _need(isinstance(t, torch.Tensor) and t.dtype in _T, "%s must be a float32, bfloat16 or float16 tensor", name)
-    _need(t.is_cuda, "%s is on %s: the operators run on a GPU only", name, t.device)
+    if not isinstance(t, torch.Tensor) or t.dtype not in _T:
+        raise ValueError("%s must be a float32, bfloat16 or float16 tensor" % name)
+    if not t.is_cuda:
+        raise ValueError("%s is on %s: the operators run on a GPU only" % (name, t.device))
     return t.dtype, t.device
 
 
 def _like(torch, name, t, dtype, device, shape):
-    """A tensor of the call: type, device and shape as given (None: any length), unit stride in the last axis."""
-    _need(isinstance(t, torch.Tensor) and t.dtype == dtype, "%s must be a %s tensor", name, dtype)
-    _need(t.device == device, "%s is on %s, the call on %s", name, t.device, device)
-    _need(tuple(t.shape) == tuple(shape), "%s has shape %s, expected %s", name, tuple(t.shape), tuple(shape))
-    _need(not (t.requires_grad and torch.is_grad_enabled()), "%s requires a gradient: call under torch.no_grad() and use the gradient function", name)
+    """A tensor of the call: type, device and shape as given, unit stride in the last axis."""
+    if not isinstance(t, torch.Tensor) or t.dtype != dtype:
+        raise ValueError("%s must be a %s tensor" % (name, dtype))
+    if t.device != device:
+        raise ValueError("%s is on %s, the call on %s" % (name, t.device, device))
+    if t.shape != shape:
+        raise ValueError("%s has shape %s, expected %s" % (name, tuple(t.shape), tuple(shape)))
+    if t.requires_grad and torch.is_grad_enabled():
+        raise ValueError("%s requires a gradient: call under torch.no_grad() and use the gradient function" % name)
     return t if t.stride(-1) == 1 or t.shape[-1] == 1 else t.contiguous()
 
 
 def _lens(torch, name, t, device, B):
     if t is None:
         return None
-    _need(isinstance(t, torch.Tensor) and t.dtype == torch.int32 and t.device == device and tuple(t.shape) == (B,),
-          "%s must be an int32 tensor of shape (%d,) on %s", name, B, device)
+    if not isinstance(t, torch.Tensor) or t.dtype != torch.int32 or t.device != device or t.shape != (B,):
+        raise ValueError("%s must be an int32 tensor of shape (%d,) on %s" % (name, B, device))
     return t.contiguous()
 
 
 def _ptr(t):
-    return None if t is None else t.data_ptr()
-
-
-def _stream(torch, device):
-    return torch.cuda.current_stream(device).cuda_stream
+    return 0 if t is None else t.data_ptr()
 
 
 def _workspace(torch, nbytes, device):
-    return torch.empty(nbytes, dtype=torch.uint8, device=device) if nbytes else None
-
-
-def _strides(field, t, n):
-    s = t.stride()
-    for i in range(n):
-        field[i] = s[i]
+    """Scratch memory of one call, from torch's allocator: its next user on this stream comes after the call, a captured graph owns its own."""
+    return torch.empty(nbytes, dtype=torch.uint8, device=device)
 
 
 # ---- embedding ------------------------------------------------------------------------------------------------------------------
 def _ids(torch, ids, device):
-    _need(isinstance(ids, torch.Tensor) and ids.dtype in (torch.int32, torch.int64) and ids.device == device,
-          "ids must be an int32 or int64 tensor on %s", device)
+    if not isinstance(ids, torch.Tensor) or ids.dtype not in (torch.int32, torch.int64) or ids.device != device:
+        raise ValueError("ids must be an int32 or int64 tensor on %s" % device)
     return ids.contiguous(), 4 if ids.dtype == torch.int32 else 8
 
 
@@ -91,51 +91,64 @@ def embed_lookup(ids, table, scale=1.0, zero_pad=True):
     everywhere in the reference (modules.py:38-40).  An id outside the table reads as zeros."""
     torch = _torch()
     dtype, device = _first(torch, "table", table)
-    _need(table.dim() == 2 and table.shape[0] > 0 and table.shape[1] > 0, "table must have two axes, has shape %s", tuple(table.shape))
+    if table.dim() != 2 or table.shape[0] < 1 or table.shape[1] < 1:
+        raise ValueError("table must be (vocab, units), has shape %s" % (tuple(table.shape),))
     table = _like(torch, "table", table, dtype, device, table.shape)
     ids, width = _ids(torch, ids, device)
     V, U = table.shape
-    out = torch.empty(tuple(ids.shape) + (U,), dtype=dtype, device=device)
-    _chk(_lib.load_seq().oph_seq_embed_lookup(_ptr(ids), width, ids.numel(), _ptr(table), table.stride(0), V, U, float(scale),
-                                              int(zero_pad), _T[dtype], _ptr(out), device.index, _stream(torch, device)))
+    out = table.new_empty(ids.shape + (U,))
+    _chk(_lib.load_seq().oph_seq_embed_lookup(ids.data_ptr(), width, ids.numel(), table.data_ptr(), table.stride(0), V, U, float(scale),
+                                              bool(zero_pad), _T[dtype], out.data_ptr(), device.index, _state["stream"](device.index)))
     return out
 
 
 def embed_gradient(ids, dout, vocab, scale=1.0, zero_pad=True):
     """Gradient of embed_lookup with respect to its table: dout of shape ids.shape + (units,) -> (vocab, units) of dout's type, row v =
-    scale * the sum of the dout rows whose id is v, taken in float32 in a fixed order.  Rows that no id names, ids outside the table and,
-    with zero_pad, row 0 get zeros / are left out."""
+    scale * the sum of the dout rows whose id is v, taken in float32 in a fixed order.  Rows that no id names, and with zero_pad row 0, are
+    zeros; ids outside the table are left out."""
     torch = _torch()
     dtype, device = _first(torch, "dout", dout)
     ids, width = _ids(torch, ids, device)
-    _need(dout.dim() >= 1 and dout.shape[-1] > 0, "dout must have a last axis of units, has shape %s", tuple(dout.shape))
+    if dout.dim() < 1 or dout.shape[-1] < 1:
+        raise ValueError("dout must have a last axis of units, has shape %s" % (tuple(dout.shape),))
     U = dout.shape[-1]
-    dout = _like(torch, "dout", dout, dtype, device, tuple(ids.shape) + (U,)).reshape(-1, U)
-    _need(isinstance(vocab, int) and vocab > 0, "vocab must be a positive number of rows, is %r", vocab)
-    lib = _lib.load_seq()
-    ws = _workspace(torch, _chk(lib.oph_seq_embed_workspace(ids.numel(), vocab, U)), device)
-    grad = torch.empty((vocab, U), dtype=dtype, device=device)
-    _chk(lib.oph_seq_embed_gradient(_ptr(ids), width, ids.numel(), _ptr(dout), dout.stride(0), vocab, U, float(scale), int(zero_pad),
-                                    _T[dtype], _ptr(grad), _ptr(ws), ws.numel(), device.index, _stream(torch, device)))
+    dout = _like(torch, "dout", dout, dtype, device, ids.shape + (U,))
+    if dout.dim() != 2:
+        dout = dout.reshape(-1, U)
+    if not isinstance(vocab, int) or vocab < 1:
+        raise ValueError("vocab must be a positive number of rows, is %r" % (vocab,))
+    lib, n = _lib.load_seq(), ids.numel()
+    nbytes = _chk(lib.oph_seq_embed_workspace(n, vocab, U))
+    ws = _workspace(torch, nbytes, device)
+    grad = dout.new_empty((vocab, U))
+    _chk(lib.oph_seq_embed_gradient(ids.data_ptr(), width, n, dout.data_ptr(), dout.stride(0), vocab, U, float(scale), bool(zero_pad),
+                                    _T[dtype], grad.data_ptr(), ws.data_ptr(), nbytes, device.index, _state["stream"](device.index)))
     return grad
 
 
 # ---- gated linear recurrence -----------------------------------------------------------------------------------------------------
 def _recur(torch, x, gate, h0, lengths):
     dtype, device = _first(torch, "x", x)
-    _need(x.dim() == 3 and x.shape[2] > 0, "x must be (batch, time, channels), has shape %s", tuple(x.shape))
-    B, T, Ch = x.shape
-    x = _like(torch, "x", x, dtype, device, (B, T, Ch))
-    gate = _like(torch, "gate", gate, dtype, device, (B, T, Ch))
+    if x.dim() != 3 or x.shape[2] < 1:
+        raise ValueError("x must be (batch, time, channels), has shape %s" % (tuple(x.shape),))
+    shape = x.shape
+    x = _like(torch, "x", x, dtype, device, shape)
+    gate = _like(torch, "gate", gate, dtype, device, shape)
     if h0 is not None:
-        h0 = _like(torch, "h0", h0, torch.float32, device, (B, Ch)).contiguous()
-    lens = _lens(torch, "lengths", lengths, device, B)
-    a = _lib.OphSeqRecur()
-    a.x, a.gate, a.h0, a.lens = _ptr(x), _ptr(gate), _ptr(h0), _ptr(lens)
-    _strides(a.x_stride, x, 2)
-    _strides(a.gate_stride, gate, 2)
-    a.B, a.T, a.C, a.dtype = B, T, Ch, _T[dtype]
-    return a, dtype, device, (x, gate, h0, lens)
+        h0 = _like(torch, "h0", h0, torch.float32, device, (shape[0], shape[2])).contiguous()
+    return dtype, device, shape, x, gate, h0, _lens(torch, "lengths", lengths, device, shape[0])
+
+
+def _run_recur(torch, call, gradient, pointers, strides, shape, dtype, device):
+    """Fills the argument structure (include/ophelia_seq.h: oph_seq_recur), finds the workspace and makes the call."""
+    lib = _lib.load_seq()
+    sizes = tuple(shape) + (_T[dtype],)
+    a = _RECUR.pack(*pointers, *strides, 0, 0, *sizes)
+    nbytes = _chk(lib.oph_seq_recur_workspace(a, gradient))
+    if nbytes:
+        ws = _workspace(torch, nbytes, device)
+        a = _RECUR.pack(*pointers, *strides, ws.data_ptr(), nbytes, *sizes)
+    _chk(call(a, device.index, _state["stream"](device.index)))
 
 
 def gated_recurrence(x, gate, h0=None, lengths=None):
@@ -143,64 +156,61 @@ def gated_recurrence(x, gate, h0=None, lengths=None):
     of x's type and the state after the last step, (B, C) float32, which the next call takes as h0 (T = 1: one decoder step).
     lengths (B) int32: steps at or past a sequence's length are not read, keep its state and have h = 0."""
     torch = _torch()
-    a, dtype, device, keep = _recur(torch, x, gate, h0, lengths)
-    h = torch.empty((a.B, a.T, a.C), dtype=dtype, device=device)
-    last = torch.empty((a.B, a.C), dtype=torch.float32, device=device)
-    a.h, a.h_last = _ptr(h), _ptr(last)
-    lib = _lib.load_seq()
-    ws = _workspace(torch, _chk(lib.oph_seq_recur_workspace(C.byref(a), 0)), device)
-    if ws is not None:
-        a.workspace, a.workspace_bytes = _ptr(ws), ws.numel()
-    _chk(lib.oph_seq_recur_forward(C.byref(a), device.index, _stream(torch, device)))
+    dtype, device, shape, x, gate, h0, lens = _recur(torch, x, gate, h0, lengths)
+    h = x.new_empty(shape)
+    last = x.new_empty((shape[0], shape[2]), dtype=torch.float32)
+    _run_recur(torch, _lib.load_seq().oph_seq_recur_forward, 0,
+               (x.data_ptr(), gate.data_ptr(), _ptr(h0), h.data_ptr(), last.data_ptr(), 0, 0, 0, 0, 0, _ptr(lens)),
+               x.stride()[:2] + gate.stride()[:2] + (0, 0, 0, 0), shape, dtype, device)
     return h, last
 
 
 def gated_recurrence_gradient(dh, x, gate, h, h0=None, dh_last=None, lengths=None):
     """Gradient of gated_recurrence: dh (B, T, C) and dh_last (B, C) float32 or None are the gradients of its two results, h its first
-    result.  Returns dx, dgate (B, T, C) and dh0 (B, C) float32; all three are 0 past a sequence's length (dh0 = dh_last for length 0)."""
+    result.  Returns dx, dgate (B, T, C), 0 past a sequence's length, and dh0 (B, C) float32 (dh_last for a sequence of length 0)."""
     torch = _torch()
-    a, dtype, device, keep = _recur(torch, x, gate, h0, lengths)
-    shape = (a.B, a.T, a.C)
+    dtype, device, shape, x, gate, h0, lens = _recur(torch, x, gate, h0, lengths)
     dh, h = _like(torch, "dh", dh, dtype, device, shape), _like(torch, "h", h, dtype, device, shape)
+    state = (shape[0], shape[2])
     if dh_last is not None:
-        dh_last = _like(torch, "dh_last", dh_last, torch.float32, device, shape[::2]).contiguous()
-    dx, dgate = torch.empty(shape, dtype=dtype, device=device), torch.empty(shape, dtype=dtype, device=device)
-    dh0 = torch.empty(shape[::2], dtype=torch.float32, device=device)
-    a.h, a.dh, a.dh_last, a.dx, a.dgate, a.dh0 = _ptr(h), _ptr(dh), _ptr(dh_last), _ptr(dx), _ptr(dgate), _ptr(dh0)
-    _strides(a.h_stride, h, 2)
-    _strides(a.dh_stride, dh, 2)
-    lib = _lib.load_seq()
-    ws = _workspace(torch, _chk(lib.oph_seq_recur_workspace(C.byref(a), 1)), device)
-    if ws is not None:
-        a.workspace, a.workspace_bytes = _ptr(ws), ws.numel()
-    _chk(lib.oph_seq_recur_gradient(C.byref(a), device.index, _stream(torch, device)))
+        dh_last = _like(torch, "dh_last", dh_last, torch.float32, device, state).contiguous()
+    dx, dgate, dh0 = x.new_empty(shape), x.new_empty(shape), x.new_empty(state, dtype=torch.float32)
+    _run_recur(torch, _lib.load_seq().oph_seq_recur_gradient, 1,
+               (x.data_ptr(), gate.data_ptr(), _ptr(h0), h.data_ptr(), 0, dh.data_ptr(), _ptr(dh_last), dx.data_ptr(), dgate.data_ptr(),
+                dh0.data_ptr(), _ptr(lens)),
+               x.stride()[:2] + gate.stride()[:2] + h.stride()[:2] + dh.stride()[:2], shape, dtype, device)
     return dx, dgate, dh0
 
 
 # ---- cross attention ---------------------------------------------------------------------------------------------------------------
 def _attention(torch, q, k, v, q_lens, k_lens, key_mask, scale):
     dtype, device = _first(torch, "q", q)
-    _need(q.dim() == 4, "q must be (batch, time, heads, head size), has shape %s", tuple(q.shape))
-    _need(isinstance(k, torch.Tensor) and k.dim() == 4, "k must be (batch, time, heads, head size)")
+    if q.dim() != 4:
+        raise ValueError("q must be (batch, time, heads, head size), has shape %s" % (tuple(q.shape),))
+    if not isinstance(k, torch.Tensor) or k.dim() != 4:
+        raise ValueError("k must be (batch, time, heads, head size)")
     B, Tq, Hq, D = q.shape
     Tk, Hk = k.shape[1], k.shape[2]
-    q = _like(torch, "q", q, dtype, device, (B, Tq, Hq, D))
-    k = _like(torch, "k", k, dtype, device, (B, Tk, Hk, D))
-    v = _like(torch, "v", v, dtype, device, (B, Tk, Hk, D))
+    shape = (B, Tk, Hk, D)
+    q = _like(torch, "q", q, dtype, device, q.shape)
+    k, v = _like(torch, "k", k, dtype, device, shape), _like(torch, "v", v, dtype, device, shape)
     ql, kl = _lens(torch, "q_lens", q_lens, device, B), _lens(torch, "k_lens", k_lens, device, B)
-    a = _lib.OphSeqAttn()
-    if key_mask is not None:
-        _need(isinstance(key_mask, torch.Tensor) and key_mask.dtype in (torch.bool, torch.uint8) and key_mask.device == device and
-              tuple(key_mask.shape) == (B, Tk), "key_mask must be a bool tensor of shape (%d, %d) on %s", B, Tk, device)
-        a.mask = _ptr(key_mask)
-        _strides(a.mask_stride, key_mask, 2)
-    a.q, a.k, a.v, a.q_lens, a.k_lens = _ptr(q), _ptr(k), _ptr(v), _ptr(ql), _ptr(kl)
-    _strides(a.q_stride, q, 3)
-    _strides(a.k_stride, k, 3)
-    _strides(a.v_stride, v, 3)
-    a.B, a.Tq, a.Tk, a.Hq, a.Hk, a.D, a.dtype = B, Tq, Tk, Hq, Hk, D, _T[dtype]
-    a.scale = 1.0 / math.sqrt(D) if scale is None and D else float(scale or 0.0)
-    return a, dtype, device, (q, k, v, ql, kl)
+    if key_mask is not None and (not isinstance(key_mask, torch.Tensor) or key_mask.dtype not in (torch.bool, torch.uint8) or
+                                 key_mask.device != device or key_mask.shape != (B, Tk)):
+        raise ValueError("key_mask must be a bool tensor of shape (%d, %d) on %s" % (B, Tk, device))
+    sizes = (B, Tq, Tk, Hq, Hk, D, _T[dtype], D ** -0.5 if scale is None and D else float(scale or 0.0))
+    return dtype, device, q, k, v, ql, kl, sizes
+
+
+def _run_attention(torch, call, gradient, pointers, strides, sizes, device):
+    """Fills the argument structure (include/ophelia_seq.h: oph_seq_attn), finds the workspace and makes the call."""
+    lib = _lib.load_seq()
+    a = _ATTN.pack(*pointers, *strides, 0, 0, *sizes)
+    nbytes = _chk(lib.oph_seq_attn_workspace(a, gradient))
+    if nbytes:
+        ws = _workspace(torch, nbytes, device)
+        a = _ATTN.pack(*pointers, *strides, ws.data_ptr(), nbytes, *sizes)
+    _chk(call(a, device.index, _state["stream"](device.index)))
 
 
 def cross_attention(q, k, v, q_lens=None, k_lens=None, key_mask=None, scale=None):
@@ -210,16 +220,13 @@ def cross_attention(q, k, v, q_lens=None, k_lens=None, key_mask=None, scale=None
     excluded is never used, NaN included.  Returns out (B, Tq, Hq, D) and lse (B, Hq, Tq) float32, the logarithm of each row's sum of
     exponentials: exp(scale * q k^T - lse) are the alignments.  A row without key or query has out = 0 and lse = -inf."""
     torch = _torch()
-    a, dtype, device, keep = _attention(torch, q, k, v, q_lens, k_lens, key_mask, scale)
-    lib = _lib.load_seq()
-    nbytes = _chk(lib.oph_seq_attn_workspace(C.byref(a), 0))
-    out = torch.empty((a.B, a.Tq, a.Hq, a.D), dtype=dtype, device=device)
-    lse = torch.empty((a.B, a.Hq, a.Tq), dtype=torch.float32, device=device)
-    ws = _workspace(torch, nbytes, device)
-    a.out, a.lse = _ptr(out), _ptr(lse)
-    if ws is not None:
-        a.workspace, a.workspace_bytes = _ptr(ws), ws.numel()
-    _chk(lib.oph_seq_attn_forward(C.byref(a), device.index, _stream(torch, device)))
+    dtype, device, q, k, v, ql, kl, sizes = _attention(torch, q, k, v, q_lens, k_lens, key_mask, scale)
+    out = q.new_empty(q.shape)
+    lse = q.new_empty((sizes[0], sizes[3], sizes[1]), dtype=torch.float32)
+    mask = (0, 0) if key_mask is None else key_mask.stride()
+    _run_attention(torch, _lib.load_seq().oph_seq_attn_forward, 0,
+                   (q.data_ptr(), k.data_ptr(), v.data_ptr(), out.data_ptr(), lse.data_ptr(), 0, 0, 0, 0, _ptr(ql), _ptr(kl), _ptr(key_mask)),
+                   q.stride()[:3] + k.stride()[:3] + v.stride()[:3] + _NO_STRIDES + mask, sizes, device)
     return out, lse
 
 
@@ -228,19 +235,14 @@ def cross_attention_gradient(dout, q, k, v, out, lse, q_lens=None, k_lens=None, 
     Returns dq, dk, dv in the shapes of q, k, v, zero for queries and keys that took no part; k and v heads shared by several query
     heads get the sum over them, expanded (broadcast) inputs the gradient of every copy."""
     torch = _torch()
-    a, dtype, device, keep = _attention(torch, q, k, v, q_lens, k_lens, key_mask, scale)
-    shape = (a.B, a.Tq, a.Hq, a.D)
-    dout = _like(torch, "dout", dout, dtype, device, shape)
-    out = _like(torch, "out", out, dtype, device, shape).contiguous()
-    lse = _like(torch, "lse", lse, torch.float32, device, (a.B, a.Hq, a.Tq)).contiguous()
-    lib = _lib.load_seq()
-    nbytes = _chk(lib.oph_seq_attn_workspace(C.byref(a), 1))
-    dq = torch.empty(shape, dtype=dtype, device=device)
-    dk, dv = (torch.empty((a.B, a.Tk, a.Hk, a.D), dtype=dtype, device=device) for _ in range(2))
-    ws = _workspace(torch, nbytes, device)
-    a.out, a.lse, a.dout, a.dq, a.dk, a.dv = _ptr(out), _ptr(lse), _ptr(dout), _ptr(dq), _ptr(dk), _ptr(dv)
-    _strides(a.dout_stride, dout, 3)
-    if ws is not None:
-        a.workspace, a.workspace_bytes = _ptr(ws), ws.numel()
-    _chk(lib.oph_seq_attn_gradient(C.byref(a), device.index, _stream(torch, device)))
+    dtype, device, q, k, v, ql, kl, sizes = _attention(torch, q, k, v, q_lens, k_lens, key_mask, scale)
+    dout = _like(torch, "dout", dout, dtype, device, q.shape)
+    out = _like(torch, "out", out, dtype, device, q.shape).contiguous()
+    lse = _like(torch, "lse", lse, torch.float32, device, (sizes[0], sizes[3], sizes[1])).contiguous()
+    dq, dk, dv = q.new_empty(q.shape), q.new_empty(k.shape), q.new_empty(k.shape)
+    mask = (0, 0) if key_mask is None else key_mask.stride()
+    _run_attention(torch, _lib.load_seq().oph_seq_attn_gradient, 1,
+                   (q.data_ptr(), k.data_ptr(), v.data_ptr(), out.data_ptr(), lse.data_ptr(), dout.data_ptr(), dq.data_ptr(), dk.data_ptr(),
+                    dv.data_ptr(), _ptr(ql), _ptr(kl), _ptr(key_mask)),
+                   q.stride()[:3] + k.stride()[:3] + v.stride()[:3] + dout.stride()[:3] + mask, sizes, device)
     return dq, dk, dv

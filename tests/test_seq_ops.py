@@ -117,3 +117,13 @@ def test_product_sources_of_the_operators_stand_alone():
     src = open(os.path.join(ROOT, "ophelia_amd", "device_ops.py")).read()
     assert "oracle" not in src
     assert "-packed-fp32-ops" in open(os.path.join(ROOT, "ophelia_amd", "_lib.py")).read()
+
+
+def test_packed_arguments_match_the_structures():
+    from ophelia_amd import _lib, device_ops
+    assert device_ops._ATTN.size == C.sizeof(_lib.OphSeqAttn) and device_ops._RECUR.size == C.sizeof(_lib.OphSeqRecur)
+    a = _lib.OphSeqAttn.from_buffer_copy(device_ops._ATTN.pack(*range(12), *range(100, 114), 200, 201, *range(300, 307), 0.5))
+    assert (a.q or 0, a.mask, list(a.q_stride), list(a.dout_stride), list(a.mask_stride)) == (0, 11, [100, 101, 102], [109, 110, 111], [112, 113])
+    assert (a.workspace, a.workspace_bytes, a.B, a.Hk, a.dtype, a.scale) == (200, 201, 300, 304, 306, 0.5)
+    r = _lib.OphSeqRecur.from_buffer_copy(device_ops._RECUR.pack(*range(11), *range(100, 108), 200, 201, *range(300, 304)))
+    assert (r.gate, r.lens, list(r.dh_stride), r.workspace, r.workspace_bytes, r.B, r.dtype) == (1, 10, [106, 107], 200, 201, 300, 303)
