@@ -119,10 +119,10 @@ def embed_gradient(ids, dout, vocab, scale=1.0, zero_pad=True):
         raise ValueError("vocab must be a positive number of rows, is %r" % (vocab,))
     lib, n = _lib.load_seq(), ids.numel()
     nbytes = _chk(lib.oph_seq_embed_workspace(n, vocab, U))
-    ws = _workspace(torch, nbytes, device)
+    ws = _workspace(torch, nbytes, device) if nbytes else None
     grad = dout.new_empty((vocab, U))
     _chk(lib.oph_seq_embed_gradient(ids.data_ptr(), width, n, dout.data_ptr(), dout.stride(0), vocab, U, float(scale), bool(zero_pad),
-                                    _T[dtype], grad.data_ptr(), ws.data_ptr(), nbytes, device.index, _state["stream"](device.index)))
+                                    _T[dtype], grad.data_ptr(), _ptr(ws), nbytes, device.index, _state["stream"](device.index)))
     return grad
 
 

@@ -194,7 +194,7 @@ def test_attention_infinite_and_nan_inputs_stay_visible():
 
 
 # ---- embedding -----------------------------------------------------------------------------------------------------------------------
-EMBED = [(1, 1, 1), (5, 2, 3), (33, 57, 128), (2400, 57, 128), (1000, 300, 37), (4097, 70000, 8), (5000, 3, 520), (3000, 300000, 4)]
+EMBED = [(4096, 64, 72), (4097, 300, 72), (9000, 700, 100), (40000, 40, 24), (1, 1, 1), (5, 2, 3), (33, 57, 128), (2400, 57, 128), (1000, 300, 37), (4097, 70000, 8), (5000, 3, 520), (3000, 300000, 4)]
 
 
 @dtypes
@@ -216,7 +216,7 @@ def test_embed(n, V, U, idt, dt):
 
 def test_embed_all_tokens_alike_and_none():
     from ophelia_amd import modules as M
-    for n in (64, 31, 32, 33, 20000):
+    for n in (1, 7, 8, 9, 64, 31, 33, 5000, 8192, 8193, 20000):
         ids, dout = torch.full((n,), 7, dtype=torch.int32), _rand(3, (n, 48), torch.bfloat16)
         ref, bound = O.embed_gradient(ids, dout, 9)
         _within("gradient", M.embed_gradient(ids.cuda(), dout.cuda(), 9), ref, bound)

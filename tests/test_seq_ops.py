@@ -71,8 +71,9 @@ def test_embedding_refusals(lib, args, word):
 
 
 def test_embedding_workspace_is_checked(lib):
-    ok = (4096, 4, 500, 4096, 8, 5, 8, 1.0, 1, 0, 4096)
-    need = lib.oph_seq_embed_workspace(500, 5, 8)
+    ok = (4096, 4, 500, 4096, 8, 5000, 8, 1.0, 1, 0, 4096)
+    need = lib.oph_seq_embed_workspace(500, 5000, 8)
+    assert need > 0
     for ws, size in ((None, need), (4096, need - 1), (4104, need)):
         assert lib.oph_seq_embed_gradient(*ok, ws, size, 0, None) == -1 and "workspace" in lib.oph_seq_last_error().decode()
 
