@@ -1,10 +1,11 @@
 // Cross attention in fp32 for problems that do not fill the machine with 128-row workgroups: forward and gradient on 16x16x4 products.
 //
 // The fp32 matrix rate is a sixteenth of the 16-bit one, so a tile's time is its products' and not its loads': operands come straight from
-// memory (row pieces of 64 bytes, columns of 64 bytes), no tile is shared through LDS.  A workgroup owns 16 rows (forward, dq) or 16
-// keys (dk, dv) and its 4 waves take every fourth tile of 16 of the other axis; their results meet in LDS in the order of the waves.
-// 16 instead of 32 rows halve both the work of a partly filled tile and the registers of D = 256: all operands and results of a
-// tile are resident (forward 4, dq 5, dk + dv 6 times 64 registers).
+// memory (row pieces of 64 bytes, columns of 64 bytes), no tile of the other axis is shared through LDS.  A workgroup owns 16 rows
+// (forward, dq) or 16 keys (dk, dv), whose operands its NW waves share in LDS; every wave takes every NW-th tile of 16 of the other axis, and
+// their results are added in a fixed order at the end.  16 instead of 32 rows halve both the work of a partly filled tile and the
+// registers of D = 256: with the shared operands in LDS the waves (4, or 8 where two fit a SIMD) have room for their results and for
+// two tiles x and y of what comes from memory: as soon as the products that read one are issued it takes its next load, a product ahead of its next use.
 //
 // Layout of a 16x16 product: lane l holds column l % 16 and rows 4(l/16) + j in register j; as the operand of the next product register j
 // is the element of step j, which contracts rows {j, 4 + j, 8 + j, 12 + j}, and the other operand is read in the same order.
@@ -21,24 +22,38 @@ __device__ __forceinline__ f32x4 mma16(const f32x4& a, const f32x4& b, f32x4 c) 
 }
 __device__ __forceinline__ f32x4 loadf4(const float* p) { return __builtin_bit_cast(f32x4, load16(p)); }
 
-// a row's operand: elements 16s + 4(l/16) .. + 3, zeros where !ok and beyond D
-template <int DP> __device__ __forceinline__ void rows16(f32x4 (&f)[DP / 16], const float* row, int D, bool ok, int g) {
+// A row's operand: elements 16s + 4(l/16) .. + 3.  EXACT: D == DP; otherwise what lies beyond D is not the row's, and edge16() clears it
+// before its use.
+template <int DP, bool EXACT> __device__ __forceinline__ void rows16(f32x4 (&f)[DP / 16], const float* row, int D, int g) {
 #pragma unroll
-    for (int s = 0; s < DP / 16; ++s) {
-        const int d = 16 * s + 4 * g;
-        const f32x4 x = loadf4(row + (d < D ? d : 0));
-        f[s] = ok && d < D ? x : f32x4{0.f, 0.f, 0.f, 0.f};
+    for (int s = 0; s < DP / 16; ++s) f[s] = loadf4(row + (EXACT || 16 * s + 4 * g < D ? 16 * s + 4 * g : 0));
+}
+template <int DP, bool EXACT> __device__ __forceinline__ void edge16(f32x4 (&f)[DP / 16], int D, int g) {
+    if (!EXACT)
+#pragma unroll
+        for (int s = 0; s < DP / 16; ++s) f[s] = 16 * s + 4 * g < D ? f[s] : f32x4{0.f, 0.f, 0.f, 0.f};
+}
+// 16 rows shared in LDS as operands: cleared where !ok and beyond D
+template <int DP, int NW, class F> __device__ __forceinline__ void share16(float* tile, F row, uint32_t bits, int D) {
+#pragma unroll
+    for (int i = 0; i < (16 * (DP / 4) + 64 * NW - 1) / (64 * NW); ++i) {
+        const int c = i * 64 * NW + threadIdx.x, r = c / (DP / 4), d = c % (DP / 4) * 4;
+        if (16 * (DP / 4) % (64 * NW) && r >= 16) break;
+        const f32x4 x = loadf4(row(r) + (d < D ? d : 0));
+        *(f32x4*)(tile + r * (DP + 4) + d) = d < D && ((bits >> r) & 1) ? x : f32x4{0.f, 0.f, 0.f, 0.f};
     }
 }
-// the transposed operand: element j is column 16s + l%16 of the row that ptr[j] points to
-template <int DP> __device__ __forceinline__ void cols16(f32x4 (&f)[DP / 16], const float* const (&ptr)[4], int D, int col) {
-#pragma unroll
-    for (int s = 0; s < DP / 16; ++s) {
-        const int d = 16 * s + col < D ? 16 * s + col : 0;              // columns beyond D are results that nobody stores
-#pragma unroll
-        for (int j = 0; j < 4; ++j) f[s][j] = ptr[j][d];
-    }
+template <int DP> __device__ __forceinline__ f32x4 shared16(const float* tile, int s, int col, int g) {
+    return *(const f32x4*)(tile + col * (DP + 4) + 16 * s + 4 * g);
 }
+// the transposed operand: element j is column 16s + l%16 of the row that ptr[j] points to; columns beyond D are results that nobody stores
+template <int DP, bool EXACT> __device__ __forceinline__ void cols16(f32x4 (&f)[DP / 16], const float* const (&ptr)[4], int D, int col) {
+#pragma unroll
+    for (int s = 0; s < DP / 16; ++s)
+#pragma unroll
+        for (int j = 0; j < 4; ++j) f[s][j] = ptr[j][EXACT || 16 * s + col < D ? 16 * s + col : 0];
+}
+__device__ __forceinline__ uint32_t bits_below(int n) { return n >= 16 ? 0xffffu : n > 0 ? (1u << n) - 1 : 0; }
 template <int N> __device__ __forceinline__ void keep16(f32x4 (&f)[N], uint32_t bits, int g) {      // rows without their bit may be NaN
 #pragma unroll
     for (int s = 0; s < N; ++s)
@@ -54,16 +69,27 @@ __device__ __forceinline__ float over_groups(float x, bool max) {       // over 
     return x;
 }
 
-// results (columns of 16 x D of the four waves) -> row-major in LDS -> sums of the waves, four columns of D at a time to `out(row, d, sum)`
-template <int DP, class F> __device__ __forceinline__ void meet16(float* lds, const f32x4 (&x)[DP / 16], float weight, F out) {
+// results (columns of 16 x D of the waves) -> sums, four columns of D at a time to `out(row, d, sum)`: waves 4..7, if there, are added to 0..3
+// first, then those in their order.  All waves are past their last use of `lds`.
+template <int DP, int NW, class F> __device__ __forceinline__ void meet16(float* lds, f32x4 (&x)[DP / 16], float weight, F out) {
     constexpr int LD = DP + 4;
     const int tid = threadIdx.x, lane = tid & 63, wave = tid >> 6, g = lane >> 4, col = lane & 15;
+    float* at = lds + ((wave & 3) * 16 + col) * LD + 4 * g;
+    if (NW == 8) {
+        if (wave >= 4)
 #pragma unroll
-    for (int s = 0; s < DP / 16; ++s) *(f32x4*)(lds + (wave * 16 + col) * LD + 16 * s + 4 * g) = x[s] * weight;
+            for (int s = 0; s < DP / 16; ++s) *(f32x4*)(at + 16 * s) = x[s] * weight;
+        __syncthreads();
+        if (wave < 4)
+#pragma unroll
+            for (int s = 0; s < DP / 16; ++s) *(f32x4*)(at + 16 * s) = x[s] * weight + *(const f32x4*)(at + 16 * s);
+    } else {
+#pragma unroll
+        for (int s = 0; s < DP / 16; ++s) *(f32x4*)(at + 16 * s) = x[s] * weight;
+    }
     __syncthreads();
-#pragma unroll
-    for (int i = 0; i < DP / 64; ++i) {
-        const int c = i * 256 + tid, row = c / (DP / 4), d = c % (DP / 4) * 4;
+    for (int c = tid; c < 16 * (DP / 4); c += 64 * NW) {
+        const int row = c / (DP / 4), d = c % (DP / 4) * 4;
         f32x4 sum = *(const f32x4*)(lds + row * LD + d);
 #pragma unroll
         for (int w = 1; w < 4; ++w) sum += *(const f32x4*)(lds + (w * 16 + row) * LD + d);
@@ -71,9 +97,9 @@ template <int DP, class F> __device__ __forceinline__ void meet16(float* lds, co
     }
 }
 
-template <int DP> __global__ __launch_bounds__(256) void attn16_forward(const AttnP p) {
+template <int DP, bool EXACT, int NW> __global__ __launch_bounds__(64 * NW) void attn16_forward(const AttnP p) {
     __shared__ __attribute__((aligned(16))) float lds[64 * (DP + 4)];
-    __shared__ float ml[4][16][2];
+    __shared__ float ml[NW][16][2];
     const int tid = threadIdx.x, lane = tid & 63, wave = tid >> 6, g = lane >> 4, col = lane & 15;
     const int M = p.Tq * p.G, tiles = (M + 15) / 16;
     const int lin = on_xcd(blockIdx.x, tiles * p.B * p.Hk * p.nsplit), split = lin % p.nsplit;
@@ -82,27 +108,33 @@ template <int DP> __global__ __launch_bounds__(256) void attn16_forward(const At
     const float c = p.scale * LOG2E;
     const int per = ((w.klen + 15) / 16 + p.nsplit - 1) / p.nsplit * 16;
     const int kbeg = split * per, kend = row_time(p, row0) < w.qlen ? min(w.klen, kbeg + per) : kbeg;
-    f32x4 Q[DP / 16], O[DP / 16];
-    {
-        const int r = row0 + col;
-        rows16<DP>(Q, row_ptr<float>(p, p.q, w, r, p.qs[0], p.qs[1], p.qs[2]), p.D, r < M && row_time(p, r) < w.qlen, g);
-    }
-#pragma unroll
-    for (int s = 0; s < DP / 16; ++s) O[s] = f32x4{};
-    float m = -INFINITY, l = 0.f;
     const float* k = (const float*)p.k + w.b * p.ks[0] + w.hk * p.ks[2];
     const float* v = (const float*)p.v + w.b * p.vs[0] + w.hk * p.vs[2];
-    for (int key0 = kbeg + wave * 16; key0 < kend; key0 += 64) {
-        const uint32_t bits = (uint32_t)key_bits(p, w, key0, kend, lane) & 0xffffu;
-        if (!bits) continue;
-        f32x4 K[DP / 16], V[DP / 16], S = {};
-        rows16<DP>(K, k + (int64_t)min(key0 + col, kend - 1) * p.ks[1], p.D, true, g);
+    f32x4 O[DP / 16], x[DP / 16], y[DP / 16];                            // x: rows of keys, y: columns of values
+    auto fetch_k = [&](int key0) { rows16<DP, EXACT>(x, k + (int64_t)min(key0 + col, kend - 1) * p.ks[1], p.D, g); };
+    auto fetch_v = [&](int key0) {
         const float* at[4];
 #pragma unroll
         for (int j = 0; j < 4; ++j) at[j] = v + (int64_t)min(key0 + 4 * g + j, kend - 1) * p.vs[1];
-        cols16<DP>(V, at, p.D, col);
+        cols16<DP, EXACT>(y, at, p.D, col);
+    };
+    int key0 = kbeg + wave * 16;
+    if (key0 < kend) {
+        fetch_k(key0);
+        fetch_v(key0);
+    }
+    share16<DP, NW>(lds, [&](int i) { return row_ptr<float>(p, p.q, w, row0 + i, p.qs[0], p.qs[1], p.qs[2]); }, bits_below(min(M, w.qlen * p.G) - row0), p.D);
+    __syncthreads();
 #pragma unroll
-        for (int s = 0; s < DP / 16; ++s) S = mma16(K[s], Q[s], S);
+    for (int s = 0; s < DP / 16; ++s) O[s] = f32x4{};
+    float m = -INFINITY, l = 0.f;
+    for (; key0 < kend; key0 += 16 * NW) {
+        const uint32_t bits = (uint32_t)key_bits(p, w, key0, kend, lane) & 0xffffu;
+        f32x4 S = {};
+        edge16<DP, EXACT>(x, p.D, g);
+#pragma unroll
+        for (int s = 0; s < DP / 16; ++s) S = mma16(x[s], shared16<DP>(lds, s, col, g), S);
+        if (key0 + 16 * NW < kend) fetch_k(key0 + 16 * NW);
         float top = -INFINITY;
 #pragma unroll
         for (int j = 0; j < 4; ++j) {
@@ -123,25 +155,26 @@ template <int DP> __global__ __launch_bounds__(256) void attn16_forward(const At
 #pragma unroll
             for (int s = 0; s < DP / 16; ++s) O[s] *= shrink;
         }
-        if (bits != 0xffffu) keep16(V, bits, g);
+        if (bits != 0xffffu) keep16(y, bits, g);
 #pragma unroll
-        for (int s = 0; s < DP / 16; ++s) O[s] = mma16(V[s], S, O[s]);
+        for (int s = 0; s < DP / 16; ++s) O[s] = mma16(y[s], S, O[s]);
+        if (key0 + 16 * NW < kend) fetch_v(key0 + 16 * NW);
     }
     l = over_groups(l, false);
     if (g == 0) { ml[wave][col][0] = m; ml[wave][col][1] = l; }
     __syncthreads();
     float top = -INFINITY;
 #pragma unroll
-    for (int i = 0; i < 4; ++i) top = fmaxf(top, ml[i][col][0]);
+    for (int i = 0; i < NW; ++i) top = fmaxf(top, ml[i][col][0]);
     const int64_t unit = ((int64_t)(w.b * p.Hk + w.hk) * tiles + w.tile) * p.nsplit + split;
-    meet16<DP>(lds, O, exp2_(m - (top == -INFINITY ? 0.f : top)), [&](int row, int d, f32x4 o) {
+    meet16<DP, NW>(lds, O, exp2_(m - (top == -INFINITY ? 0.f : top)), [&](int row, int d, f32x4 o) {
         const int r = row0 + row, t = row_time(p, r), h = w.hk * p.G + r - t * p.G;
         if (r >= M || d >= p.D) return;
         float om = -INFINITY, ol = 0.f;
 #pragma unroll
-        for (int i = 0; i < 4; ++i) om = fmaxf(om, ml[i][row][0]);
+        for (int i = 0; i < NW; ++i) om = fmaxf(om, ml[i][row][0]);
 #pragma unroll
-        for (int i = 0; i < 4; ++i) ol += ml[i][row][1] * exp2_(ml[i][row][0] - (om == -INFINITY ? 0.f : om));
+        for (int i = 0; i < NW; ++i) ol += ml[i][row][1] * exp2_(ml[i][row][0] - (om == -INFINITY ? 0.f : om));
         if (p.nsplit == 1) {
             const bool live = t < w.qlen && ol != 0.f;
             store4<float>((float*)p.o0 + (((int64_t)w.b * p.Tq + t) * (p.Hk * p.G) + h) * p.D + d, live ? o * (1.f / ol) : f32x4{0.f, 0.f, 0.f, 0.f});
@@ -153,7 +186,7 @@ template <int DP> __global__ __launch_bounds__(256) void attn16_forward(const At
     });
 }
 
-template <int DP> __global__ __launch_bounds__(256) void attn16_dq(const AttnP p) {
+template <int DP, bool EXACT, int NW> __global__ __launch_bounds__(64 * NW) void attn16_dq(const AttnP p) {
     __shared__ __attribute__((aligned(16))) float lds[64 * (DP + 4)];
     const int tid = threadIdx.x, lane = tid & 63, wave = tid >> 6, g = lane >> 4, col = lane & 15;
     const int M = p.Tq * p.G, Hq = p.Hk * p.G, tiles = (M + 15) / 16;
@@ -164,16 +197,33 @@ template <int DP> __global__ __launch_bounds__(256) void attn16_dq(const AttnP p
     const float c = p.scale * LOG2E;
     const int per = ((w.klen + 15) / 16 + p.nsplit - 1) / p.nsplit * 16;
     const int kbeg = split * per, kend = row_time(p, row0) < w.qlen ? min(w.klen, kbeg + per) : kbeg;
-    f32x4 Q[DP / 16], dO[DP / 16], dQ[DP / 16];
-    rows16<DP>(Q, row_ptr<float>(p, p.q, w, r, p.qs[0], p.qs[1], p.qs[2]), p.D, row, g);
-    rows16<DP>(dO, row_ptr<float>(p, p.dout, w, r, p.ds[0], p.ds[1], p.ds[2]), p.D, row, g);
+    const float* k = (const float*)p.k + w.b * p.ks[0] + w.hk * p.ks[2];
+    const float* v = (const float*)p.v + w.b * p.vs[0] + w.hk * p.vs[2];
+    f32x4 dQ[DP / 16], x[DP / 16], y[DP / 16];                           // x: rows, then columns of keys, y: rows of values
+    float *tq = lds, *to = lds + 16 * (DP + 4);
+    auto fetch = [&](f32x4 (&f)[DP / 16], const float* base, int64_t stride, int key0) {
+        rows16<DP, EXACT>(f, base + (int64_t)min(key0 + col, kend - 1) * stride, p.D, g);
+    };
+    int key0 = kbeg + wave * 16;
+    if (key0 < kend) {
+        fetch(x, k, p.ks[1], key0);
+        fetch(y, v, p.vs[1], key0);
+    }
+    const uint32_t mine = bits_below(min(M, w.qlen * p.G) - row0);
+    share16<DP, NW>(tq, [&](int i) { return row_ptr<float>(p, p.q, w, row0 + i, p.qs[0], p.qs[1], p.qs[2]); }, mine, p.D);
+    share16<DP, NW>(to, [&](int i) { return row_ptr<float>(p, p.dout, w, row0 + i, p.ds[0], p.ds[1], p.ds[2]); }, mine, p.D);
+    rows16<DP, EXACT>(dQ, row_ptr<float>(p, p.out, w, r, (int64_t)p.Tq * Hq * p.D, (int64_t)Hq * p.D, p.D), p.D, g);
+    __syncthreads();
     float delta = 0.f, lse2 = INFINITY;
     {
-        rows16<DP>(dQ, row_ptr<float>(p, p.out, w, r, (int64_t)p.Tq * Hq * p.D, (int64_t)Hq * p.D, p.D), p.D, row, g);
+        edge16<DP, EXACT>(dQ, p.D, g);
 #pragma unroll
-        for (int s = 0; s < DP / 16; ++s)
+        for (int s = 0; s < DP / 16; ++s) {
+            const f32x4 d = shared16<DP>(to, s, col, g);
 #pragma unroll
-            for (int j = 0; j < 4; ++j) delta = fmaf(dQ[s][j], dO[s][j], delta);
+            for (int j = 0; j < 4; ++j) delta = fmaf(dQ[s][j], d[j], delta);
+        }
+        if (!row) delta = 0.f;
         delta = over_groups(delta, false);
         const int64_t at = ((int64_t)w.b * Hq + h) * p.Tq + t;
         if (row) {
@@ -184,30 +234,29 @@ template <int DP> __global__ __launch_bounds__(256) void attn16_dq(const AttnP p
     }
 #pragma unroll
     for (int s = 0; s < DP / 16; ++s) dQ[s] = f32x4{};
-    const float* k = (const float*)p.k + w.b * p.ks[0] + w.hk * p.ks[2];
-    const float* v = (const float*)p.v + w.b * p.vs[0] + w.hk * p.vs[2];
-    for (int key0 = kbeg + wave * 16; key0 < kend; key0 += 64) {
+    for (; key0 < kend; key0 += 16 * NW) {
         const uint32_t bits = (uint32_t)key_bits(p, w, key0, kend, lane) & 0xffffu;
-        if (!bits) continue;
-        f32x4 K[DP / 16], V[DP / 16], S = {}, dP = {};
-        const int64_t mine = min(key0 + col, kend - 1);
-        rows16<DP>(K, k + mine * p.ks[1], p.D, true, g);
-        rows16<DP>(V, v + mine * p.vs[1], p.D, true, g);
+        f32x4 S = {}, dP = {};
+        edge16<DP, EXACT>(x, p.D, g);
 #pragma unroll
-        for (int s = 0; s < DP / 16; ++s) S = mma16(K[s], Q[s], S);
+        for (int s = 0; s < DP / 16; ++s) S = mma16(x[s], shared16<DP>(tq, s, col, g), S);
         const float* at[4];
 #pragma unroll
         for (int j = 0; j < 4; ++j) at[j] = k + (int64_t)min(key0 + 4 * g + j, kend - 1) * p.ks[1];
-        cols16<DP>(K, at, p.D, col);
+        cols16<DP, EXACT>(x, at, p.D, col);
+        edge16<DP, EXACT>(y, p.D, g);
 #pragma unroll
-        for (int s = 0; s < DP / 16; ++s) dP = mma16(V[s], dO[s], dP);
+        for (int s = 0; s < DP / 16; ++s) dP = mma16(y[s], shared16<DP>(to, s, col, g), dP);
+        if (key0 + 16 * NW < kend) fetch(y, v, p.vs[1], key0 + 16 * NW);
 #pragma unroll
         for (int j = 0; j < 4; ++j) S[j] = (bits >> (4 * g + j)) & 1 ? exp2_(fmaf(S[j], c, -lse2)) * (dP[j] - delta) : 0.f;
-        if (bits != 0xffffu) keep16(K, bits, g);
+        if (bits != 0xffffu) keep16(x, bits, g);
 #pragma unroll
-        for (int s = 0; s < DP / 16; ++s) dQ[s] = mma16(K[s], S, dQ[s]);
+        for (int s = 0; s < DP / 16; ++s) dQ[s] = mma16(x[s], S, dQ[s]);
+        if (key0 + 16 * NW < kend) fetch(x, k, p.ks[1], key0 + 16 * NW);
     }
-    meet16<DP>(lds, dQ, p.scale, [&](int i, int d, f32x4 x) {
+    __syncthreads();
+    meet16<DP, NW>(lds, dQ, p.scale, [&](int i, int d, f32x4 x) {
         const int rr = row0 + i, tt = row_time(p, rr), hh = w.hk * p.G + rr - tt * p.G;
         if (rr >= M || d >= p.D) return;
         const int64_t at = (((int64_t)w.b * p.Tq + tt) * Hq + hh) * p.D + d;
@@ -217,7 +266,7 @@ template <int DP> __global__ __launch_bounds__(256) void attn16_dq(const AttnP p
     });
 }
 
-template <int DP> __global__ __launch_bounds__(256) void attn16_dkv(const AttnP p) {
+template <int DP, bool EXACT, int NW> __global__ __launch_bounds__(64 * NW) void attn16_dkv(const AttnP p) {
     __shared__ __attribute__((aligned(16))) float lds[64 * (DP + 4)];
     const int tid = threadIdx.x, lane = tid & 63, wave = tid >> 6, g = lane >> 4, col = lane & 15;
     const int Hq = p.Hk * p.G, tiles = (p.Tk + 15) / 16;
@@ -226,52 +275,63 @@ template <int DP> __global__ __launch_bounds__(256) void attn16_dkv(const AttnP 
     const int key0 = w.tile * 16;
     const uint32_t keys = (uint32_t)key_bits(p, w, key0, w.klen, lane) & 0xffffu;
     const float c = p.scale * LOG2E;
-    f32x4 K[DP / 16], V[DP / 16], dK[DP / 16], dV[DP / 16];
-    {
-        const int64_t key = min(key0 + col, p.Tk - 1);
-        const bool ok = (keys >> col) & 1;
-        rows16<DP>(K, (const float*)p.k + w.b * p.ks[0] + w.hk * p.ks[2] + key * p.ks[1], p.D, ok, g);
-        rows16<DP>(V, (const float*)p.v + w.b * p.vs[0] + w.hk * p.vs[2] + key * p.vs[1], p.D, ok, g);
-    }
-#pragma unroll
-    for (int s = 0; s < DP / 16; ++s) dK[s] = dV[s] = f32x4{};
     const int rows = keys ? w.qlen * p.G : 0;
     const int per = ((rows + 15) / 16 + p.nsplit - 1) / p.nsplit * 16;
     const int rbeg = split * per, rend = min(rows, rbeg + per);
-    for (int r0 = rbeg + wave * 16; r0 < rend; r0 += 64) {
+    f32x4 dK[DP / 16], dV[DP / 16], x[DP / 16], y[DP / 16];              // x: rows of q, columns of dout, y: rows of dout, columns of q
+    float *tk = lds, *tv = lds + 16 * (DP + 4);
+    auto q_row = [&](int r) { return row_ptr<float>(p, p.q, w, min(r, rend - 1), p.qs[0], p.qs[1], p.qs[2]); };
+    auto o_row = [&](int r) { return row_ptr<float>(p, p.dout, w, min(r, rend - 1), p.ds[0], p.ds[1], p.ds[2]); };
+    int r0 = rbeg + wave * 16;
+    if (r0 < rend) {
+        rows16<DP, EXACT>(x, q_row(r0 + col), p.D, g);
+        rows16<DP, EXACT>(y, o_row(r0 + col), p.D, g);
+    }
+    {
+        const float *k = (const float*)p.k + w.b * p.ks[0] + w.hk * p.ks[2], *v = (const float*)p.v + w.b * p.vs[0] + w.hk * p.vs[2];
+        share16<DP, NW>(tk, [&](int i) { return k + (int64_t)min(key0 + i, p.Tk - 1) * p.ks[1]; }, keys, p.D);
+        share16<DP, NW>(tv, [&](int i) { return v + (int64_t)min(key0 + i, p.Tk - 1) * p.vs[1]; }, keys, p.D);
+        __syncthreads();
+    }
+#pragma unroll
+    for (int s = 0; s < DP / 16; ++s) dK[s] = dV[s] = f32x4{};
+    for (; r0 < rend; r0 += 16 * NW) {
         const uint32_t bits = rend - r0 >= 16 ? 0xffffu : (1u << (rend - r0)) - 1;
-        f32x4 X[DP / 16], S = {}, dP = {};
+        f32x4 S = {}, dP = {};
         float lse2[4], delta[4];
         const float *qa[4], *oa[4];
 #pragma unroll
         for (int j = 0; j < 4; ++j) {
             const int r = min(r0 + 4 * g + j, rend - 1), t = row_time(p, r);
-            qa[j] = row_ptr<float>(p, p.q, w, r, p.qs[0], p.qs[1], p.qs[2]);
-            oa[j] = row_ptr<float>(p, p.dout, w, r, p.ds[0], p.ds[1], p.ds[2]);
+            qa[j] = q_row(r);
+            oa[j] = o_row(r);
             const int64_t at = ((int64_t)w.b * Hq + w.hk * p.G + r - t * p.G) * p.Tq + t;
             lse2[j] = p.lse[at];
-            lse2[j] = lse2[j] == -INFINITY ? INFINITY : lse2[j] * LOG2E;
             delta[j] = p.aux[at];
         }
-        const int mine = min(r0 + col, rend - 1);
-        rows16<DP>(X, row_ptr<float>(p, p.q, w, mine, p.qs[0], p.qs[1], p.qs[2]), p.D, true, g);
+        edge16<DP, EXACT>(x, p.D, g);
 #pragma unroll
-        for (int s = 0; s < DP / 16; ++s) S = mma16(X[s], K[s], S);
-        rows16<DP>(X, row_ptr<float>(p, p.dout, w, mine, p.ds[0], p.ds[1], p.ds[2]), p.D, true, g);
+        for (int s = 0; s < DP / 16; ++s) S = mma16(x[s], shared16<DP>(tk, s, col, g), S);
+        cols16<DP, EXACT>(x, oa, p.D, col);
+        edge16<DP, EXACT>(y, p.D, g);
 #pragma unroll
-        for (int s = 0; s < DP / 16; ++s) dP = mma16(X[s], V[s], dP);
+        for (int s = 0; s < DP / 16; ++s) dP = mma16(y[s], shared16<DP>(tv, s, col, g), dP);
+        cols16<DP, EXACT>(y, qa, p.D, col);
 #pragma unroll
-        for (int j = 0; j < 4; ++j) S[j] = (bits >> (4 * g + j)) & 1 ? exp2_(fmaf(S[j], c, -lse2[j])) : 0.f;
-        cols16<DP>(X, oa, p.D, col);
-        if (bits != 0xffffu) keep16(X, bits, g);
+        for (int j = 0; j < 4; ++j) {
+            const float l = lse2[j] == -INFINITY ? INFINITY : lse2[j] * LOG2E;
+            S[j] = (bits >> (4 * g + j)) & 1 ? exp2_(fmaf(S[j], c, -l)) : 0.f;
+        }
+        if (bits != 0xffffu) keep16(x, bits, g);
 #pragma unroll
-        for (int s = 0; s < DP / 16; ++s) dV[s] = mma16(X[s], S, dV[s]);
+        for (int s = 0; s < DP / 16; ++s) dV[s] = mma16(x[s], S, dV[s]);
+        if (r0 + 16 * NW < rend) rows16<DP, EXACT>(x, q_row(r0 + 16 * NW + col), p.D, g);
 #pragma unroll
         for (int j = 0; j < 4; ++j) S[j] = (bits >> (4 * g + j)) & 1 ? S[j] * (dP[j] - delta[j]) : 0.f;
-        cols16<DP>(X, qa, p.D, col);
-        if (bits != 0xffffu) keep16(X, bits, g);
+        if (bits != 0xffffu) keep16(y, bits, g);
 #pragma unroll
-        for (int s = 0; s < DP / 16; ++s) dK[s] = mma16(X[s], S, dK[s]);
+        for (int s = 0; s < DP / 16; ++s) dK[s] = mma16(y[s], S, dK[s]);
+        if (r0 + 16 * NW < rend) rows16<DP, EXACT>(y, o_row(r0 + 16 * NW + col), p.D, g);
     }
     const int64_t n = (int64_t)p.B * p.Tk * p.Hk * p.D;
     auto store = [&](int i, int d, f32x4 x, bool dk) {
@@ -282,16 +342,22 @@ template <int DP> __global__ __launch_bounds__(256) void attn16_dkv(const AttnP 
         float* o = p.nsplit == 1 ? (float*)(dk ? p.o1 : p.o0) : p.part + ((dk ? p.nsplit : 0) + split) * n;
         store4<float>(o + at, x);
     };
-    meet16<DP>(lds, dV, 1.f, [&](int i, int d, f32x4 x) { store(i, d, x, false); });
     __syncthreads();
-    meet16<DP>(lds, dK, p.scale, [&](int i, int d, f32x4 x) { store(i, d, x, true); });
+    meet16<DP, NW>(lds, dV, 1.f, [&](int i, int d, f32x4 x) { store(i, d, x, false); });
+    __syncthreads();
+    meet16<DP, NW>(lds, dK, p.scale, [&](int i, int d, f32x4 x) { store(i, d, x, true); });
 }
 
-template <int DP> static int go(const AttnP& p, int64_t groups, int what, void* stream) {
-    return launch<AttnP>(what == 0 ? attn16_forward<DP> : what == 1 ? attn16_dq<DP> : attn16_dkv<DP>, dim3((unsigned)groups), 256, p, 0, stream);
+template <int DP, bool EXACT> static int go(const AttnP& p, int64_t groups, int what, void* stream) {
+    constexpr int N = DP <= 128 ? 8 : 4, NKV = DP <= 64 ? 8 : 4;          // two waves a SIMD where the registers allow it
+    void (*const kernel)(AttnP) = what == 0 ? attn16_forward<DP, EXACT, N> : what == 1 ? attn16_dq<DP, EXACT, N> : attn16_dkv<DP, EXACT, NKV>;
+    return launch<AttnP>(kernel, dim3((unsigned)groups), 64 * (what == 2 ? NKV : N), p, 0, stream);
+}
+template <int DP> static int go_d(const AttnP& p, int64_t groups, int what, void* stream) {
+    return p.D == DP ? go<DP, true>(p, groups, what, stream) : go<DP, false>(p, groups, what, stream);
 }
 int attn16_launch(const AttnP& p, int64_t groups, int what, void* stream) {
-    return p.D <= 64 ? go<64>(p, groups, what, stream) : p.D <= 128 ? go<128>(p, groups, what, stream) : go<256>(p, groups, what, stream);
+    return p.D <= 64 ? go_d<64>(p, groups, what, stream) : p.D <= 128 ? go_d<128>(p, groups, what, stream) : go_d<256>(p, groups, what, stream);
 }
 
 }  // namespace ophseq

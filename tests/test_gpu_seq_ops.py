@@ -94,7 +94,7 @@ def test_attention(shape, dt):
 
 @dtypes
 @pytest.mark.parametrize("kind", ["ragged", "masked"])
-@pytest.mark.parametrize("shape", [(3, 1, 150, 2, 1, 256), (4, 40, 77, 4, 2, 64), (9, 129, 70, 32, 32, 48), (3, 5, 700, 4, 2, 128), (2, 300, 200, 2, 1, 96)], ids=str)
+@pytest.mark.parametrize("shape", [(3, 1, 150, 2, 1, 256), (4, 40, 77, 4, 2, 64), (9, 129, 70, 32, 32, 48), (3, 5, 700, 4, 2, 128), (2, 300, 200, 2, 1, 96), (2, 70, 200, 3, 1, 200)], ids=str)
 def test_attention_excluded_places_are_never_used(shape, kind, dt):
     _attend(shape, dt, kind, spoil=True)
 
