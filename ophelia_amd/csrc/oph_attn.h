@@ -24,7 +24,7 @@ struct AttnP {                       // at most 256 bytes: a larger block of arg
     int B, Tq, Tk, Hk, G, D;
     unsigned magic;                  // r / G = umulhi(r, magic) for G > 1
     float scale;
-    int nsplit;
+    int nsplit, chunk;
 };
 static_assert(sizeof(AttnP) <= 256, "AttnP");
 
@@ -32,11 +32,12 @@ struct Where { int b, hk, tile, qlen, klen; };
 
 __device__ __forceinline__ int clampi(int x, int lo, int hi) { return x < lo ? lo : x > hi ? hi : x; }
 
-// Workgroups go round robin over the 8 XCDs: every XCD gets a contiguous run of (sequence, key head, tile), so that the tiles that
-// read the same keys share an L2.
-__device__ __forceinline__ int on_xcd(int id, int n) {
-    const int q = n >> 3, r = n & 7, x = id & 7;
-    return (x < r ? x * (q + 1) : r * (q + 1) + (x - r) * q) + (id >> 3);
+// Workgroups go round robin over the 8 XCDs.  The list of (sequence, key head, tile, split) is dealt out in runs of `chunk`: long runs keep the
+// tiles that read the same keys on one L2, short ones spread sequences of different lengths over the machine (run_of()).
+__device__ __forceinline__ int on_xcd(const AttnP& p, int id, int n) {
+    if (p.chunk <= 1) return id;
+    const int round = 8 * p.chunk, x = id & 7, s = id >> 3, c = s / p.chunk;
+    return id < n / round * round ? (c * 8 + x) * p.chunk + s - c * p.chunk : id;
 }
 
 __device__ __forceinline__ Where where(const AttnP& p, int lin, int tiles) {
@@ -60,13 +61,12 @@ __device__ __forceinline__ const T* row_ptr(const AttnP& p, const void* base, co
     return (const T*)base + w.b * sb + t * st + (int64_t)(w.hk * p.G + g) * sh;
 }
 
-// bit i: key key0 + i may be attended (i < 64)
-__device__ __forceinline__ uint64_t key_bits(const AttnP& p, const Where& w, int key0, int kend, int lane) {
-    const int key = key0 + lane;
-    bool ok = key < kend;
-    if (p.mask && ok) ok = p.mask[w.b * p.ms[0] + key * p.ms[1]] != 0;
-    return __ballot(ok);
+// Which of the keys key0 + lane may be attended, in two steps: the mask's byte is loaded with (before) the keys it belongs to, and only
+// asked for when they are used.  bit i of key_bits(): key key0 + i (i < 64).
+__device__ __forceinline__ uint8_t key_byte(const AttnP& p, const Where& w, int key0, int kend, int lane) {
+    return p.mask && kend > 0 ? p.mask[w.b * p.ms[0] + min(key0 + lane, kend - 1) * p.ms[1]] : 1;
 }
+__device__ __forceinline__ uint64_t key_bits(uint8_t byte, int key0, int kend, int lane) { return __ballot(byte != 0 && key0 + lane < kend); }
 
 // the operand pieces of one row: 8 elements of every 16, by lane half; zeros where !ok and beyond D
 template <class T, int DP>
@@ -173,6 +173,7 @@ __device__ __forceinline__ void wave_lds_fence() {
 }
 
 // ---- host side -----------------------------------------------------------------------------------------------------------------
+int run_of(const oph_seq_attn* a, int64_t groups, bool few);
 int attn16_launch(const AttnP& p, int64_t groups, int what, void* stream);      // oph_attn32.hip: 0 forward, 1 dq, 2 dk and dv
 int attn_few_forward(const AttnP& p, int dtype, int64_t groups, void* stream);     // oph_attnfew.hip: M <= 4
 int attn_check(const oph_seq_attn* a, bool gradient);

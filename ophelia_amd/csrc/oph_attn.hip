@@ -54,9 +54,38 @@ __global__ __launch_bounds__(256, (wide_waves<T, DP>())) void attn_wide(const At
     __shared__ __attribute__((aligned(16))) char lds[4 * TB];
     const int tid = threadIdx.x, lane = tid & 63, wave = tid >> 6, half = lane >> 5, col = lane & 31;
     const int M = p.Tq * p.G, tiles = (M + ROWS - 1) / ROWS;
-    const Where w = where(p, on_xcd(blockIdx.x, tiles * p.B * p.Hk), tiles);
+    const Where w = where(p, on_xcd(p, blockIdx.x, tiles * p.B * p.Hk), tiles);
     const int row0 = w.tile * ROWS + wave * 32 * NQ;
     const float c = p.scale * LOG2E;
+
+    const T* k = (const T*)p.k + w.b * p.ks[0] + w.hk * p.ks[2];
+    const T* v = (const T*)p.v + w.b * p.vs[0] + w.hk * p.vs[2];
+    const bool any = row_time(p, w.tile * ROWS) < w.qlen;               // a tile of padding only: nothing to read
+    const int nt = any ? (w.klen + KT - 1) / KT : 0;
+    Stage<T, DP, KT, 256> sk, sv;
+    const T *k1 = sk.own(k, p.ks[1], p.D, tid), *v1 = sv.own(v, p.vs[1], p.D, tid);
+    uint64_t bits = 0;
+    uint8_t byte = 0;
+    auto fetch = [&](int j) {
+        const int key0 = j * KT, last = w.klen - 1;
+        byte = key_byte(p, w, key0, w.klen, lane);
+        if (key0 + KT <= w.klen) {
+            sk.load_run(k1, p.ks[1]);
+            sv.load_run(v1, p.vs[1]);
+            k1 += KT * p.ks[1];
+            v1 += KT * p.vs[1];
+            return;
+        }
+        sk.load([&](int r) { return k + (int64_t)min(key0 + r, last) * p.ks[1]; }, p.D, tid);
+        sv.load([&](int r) { return v + (int64_t)min(key0 + r, last) * p.vs[1]; }, p.D, tid);
+    };
+    auto commit = [&](int j) {
+        char* t = lds + (j & 1) * 2 * TB;
+        bits = key_bits(byte, j * KT, w.klen, lane) & (KT == 64 ? ~0ull : 0xffffffffull);
+        sk.store(t, bits, p.D, tid);
+        sv.store(t + TB, bits, p.D, tid);
+    };
+    if (nt) fetch(0);                                    // on its way while the rows' operands are loaded
 
     frag_t<T> Q[NQ][DP / 16];
     f32x16 O[NQ][DP / 32];
@@ -70,33 +99,7 @@ __global__ __launch_bounds__(256, (wide_waves<T, DP>())) void attn_wide(const At
         for (int d = 0; d < DP / 32; ++d) O[n][d] = f32x16{};
     }
 
-    const T* k = (const T*)p.k + w.b * p.ks[0] + w.hk * p.ks[2];
-    const T* v = (const T*)p.v + w.b * p.vs[0] + w.hk * p.vs[2];
-    const bool any = row_time(p, w.tile * ROWS) < w.qlen;               // a tile of padding only: nothing to read
-    const int nt = any ? (w.klen + KT - 1) / KT : 0;
-    Stage<T, DP, KT, 256> sk, sv;
-    const T *k1 = sk.own(k, p.ks[1], p.D, tid), *v1 = sv.own(v, p.vs[1], p.D, tid);
-    uint64_t bits = 0, next = 0;
-    auto fetch = [&](int j) {
-        const int key0 = j * KT, last = w.klen - 1;
-        next = key_bits(p, w, key0, w.klen, lane) & (KT == 64 ? ~0ull : 0xffffffffull);
-        if (key0 + KT <= w.klen) {
-            sk.load_run(k1, p.ks[1]);
-            sv.load_run(v1, p.vs[1]);
-            k1 += KT * p.ks[1];
-            v1 += KT * p.vs[1];
-            return;
-        }
-        sk.load([&](int r) { return k + (int64_t)min(key0 + r, last) * p.ks[1]; }, p.D, tid);
-        sv.load([&](int r) { return v + (int64_t)min(key0 + r, last) * p.vs[1]; }, p.D, tid);
-    };
-    auto commit = [&](int j) {
-        char* t = lds + (j & 1) * 2 * TB;
-        sk.store(t, next, p.D, tid);
-        sv.store(t + TB, next, p.D, tid);
-        bits = next;
-    };
-    if (nt) { fetch(0); commit(0); }
+    if (nt) commit(0);
     for (int j = 0; j < nt; ++j) {
         const uint64_t now = bits;
         __syncthreads();
@@ -175,7 +178,7 @@ __global__ __launch_bounds__(256) void attn_split(const AttnP p) {
     __shared__ float ml[4][32][2];
     const int tid = threadIdx.x, lane = tid & 63, wave = tid >> 6, half = lane >> 5, col = lane & 31;
     const int M = p.Tq * p.G, tiles = (M + 31) / 32;
-    const int lin = on_xcd(blockIdx.x, tiles * p.B * p.Hk * p.nsplit), split = lin % p.nsplit;
+    const int lin = on_xcd(p, blockIdx.x, tiles * p.B * p.Hk * p.nsplit), split = lin % p.nsplit;
     const Where w = where(p, lin / p.nsplit, tiles);
     const int row0 = w.tile * 32;
     const float c = p.scale * LOG2E;
@@ -194,8 +197,7 @@ __global__ __launch_bounds__(256) void attn_split(const AttnP p) {
     const T* k = (const T*)p.k + w.b * p.ks[0] + w.hk * p.ks[2];
     const T* v = (const T*)p.v + w.b * p.vs[0] + w.hk * p.vs[2];
     for (int key0 = kbeg + wave * 32; key0 < kend; key0 += 128) {
-        const uint64_t bits = key_bits(p, w, key0, kend, lane) & 0xffffffffull;
-        if (!bits) continue;
+        const uint8_t byte = key_byte(p, w, key0, kend, lane);
         frag_t<T> K[DP / 16];
         row_frags<T, DP>(K, k + (int64_t)min(key0 + col, kend - 1) * p.ks[1], p.D, true, half);
         f32x16 S[1] = {f32x16{}};
@@ -204,6 +206,7 @@ __global__ __launch_bounds__(256) void attn_split(const AttnP p) {
         sv.load([&](int r) { return v + (int64_t)min(key0 + r, kend - 1) * p.vs[1]; }, p.D, lane);
 #pragma unroll
         for (int s = 0; s < DP / 16; ++s) S[0] = El<T>::mma(K[s], Q[s], S[0]);
+        const uint64_t bits = key_bits(byte, key0, kend, lane) & 0xffffffffull;
         const float shrink = soft_step<1>(S, bits, st, c, half);
         if (__any(shrink != 1.f)) {
 #pragma unroll
@@ -347,6 +350,12 @@ AttnP attn_params(const oph_seq_attn* a) {
     return p;
 }
 
+// Runs of 8 where lengths differ (8 sequences of up to 2000 x 2000, 16 heads of 128: 219 us, 272 with one run an XCD; their gradient 741 and
+// 836); else, and for few rows, which share nothing, one run an XCD (a token over 8 x 16384 keys: 88 us, 94 dealt out singly).
+int run_of(const oph_seq_attn* a, int64_t groups, bool few) {
+    const int64_t run = groups / 8;
+    return (int)(!few && (a->q_lens || a->k_lens) && run > 8 ? 8 : run);
+}
 static int pad_d(int D) { return D <= 64 ? 64 : D <= 128 ? 128 : 256; }
 
 struct FwdPlan { bool few, wide; int nsplit, rows; int64_t units; };
@@ -374,12 +383,12 @@ int64_t attn_forward_workspace(const oph_seq_attn* a) {
 }
 
 template <class T, int DP, int KT, int NQ> static int forward(const oph_seq_attn* a, const FwdPlan& f, AttnP& p, void* stream) {
-    const int64_t M = (int64_t)p.Tq * p.G, heads = (int64_t)p.B * p.Hk;
-    if (f.wide) return launch<AttnP>(attn_wide<T, DP, KT, NQ>, dim3((unsigned)(cdiv(M, 128 * NQ) * heads)), 256, p, 0, stream);
+    const int64_t M = (int64_t)p.Tq * p.G, heads = (int64_t)p.B * p.Hk, groups = f.wide ? cdiv(M, 128 * NQ) * heads : f.units * f.nsplit;
+    p.chunk = run_of(a, groups, f.few);
+    if (f.wide) return launch<AttnP>(attn_wide<T, DP, KT, NQ>, dim3((unsigned)groups), 256, p, 0, stream);
     p.nsplit = f.nsplit;
     p.part = (float*)a->workspace;
     p.aux = p.part + f.units * f.nsplit * f.rows * DP;
-    const int64_t groups = f.units * f.nsplit;
     int rc;
     if (f.few) rc = attn_few_forward(p, a->dtype, groups, stream);
     else if constexpr (sizeof(T) == 4) rc = attn16_launch(p, groups, 0, stream);

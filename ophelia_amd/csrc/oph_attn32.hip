@@ -102,7 +102,7 @@ template <int DP, bool EXACT, int NW> __global__ __launch_bounds__(64 * NW) void
     __shared__ float ml[NW][16][2];
     const int tid = threadIdx.x, lane = tid & 63, wave = tid >> 6, g = lane >> 4, col = lane & 15;
     const int M = p.Tq * p.G, tiles = (M + 15) / 16;
-    const int lin = on_xcd(blockIdx.x, tiles * p.B * p.Hk * p.nsplit), split = lin % p.nsplit;
+    const int lin = on_xcd(p, blockIdx.x, tiles * p.B * p.Hk * p.nsplit), split = lin % p.nsplit;
     const Where w = where(p, lin / p.nsplit, tiles);
     const int row0 = w.tile * 16;
     const float c = p.scale * LOG2E;
@@ -119,6 +119,7 @@ template <int DP, bool EXACT, int NW> __global__ __launch_bounds__(64 * NW) void
         cols16<DP, EXACT>(y, at, p.D, col);
     };
     int key0 = kbeg + wave * 16;
+    uint8_t byte = key_byte(p, w, key0, kend, lane);
     if (key0 < kend) {
         fetch_k(key0);
         fetch_v(key0);
@@ -129,12 +130,15 @@ template <int DP, bool EXACT, int NW> __global__ __launch_bounds__(64 * NW) void
     for (int s = 0; s < DP / 16; ++s) O[s] = f32x4{};
     float m = -INFINITY, l = 0.f;
     for (; key0 < kend; key0 += 16 * NW) {
-        const uint32_t bits = (uint32_t)key_bits(p, w, key0, kend, lane) & 0xffffu;
+        const uint32_t bits = (uint32_t)key_bits(byte, key0, kend, lane) & 0xffffu;
         f32x4 S = {};
         edge16<DP, EXACT>(x, p.D, g);
 #pragma unroll
         for (int s = 0; s < DP / 16; ++s) S = mma16(x[s], shared16<DP>(lds, s, col, g), S);
-        if (key0 + 16 * NW < kend) fetch_k(key0 + 16 * NW);
+        if (key0 + 16 * NW < kend) {
+            byte = key_byte(p, w, key0 + 16 * NW, kend, lane);
+            fetch_k(key0 + 16 * NW);
+        }
         float top = -INFINITY;
 #pragma unroll
         for (int j = 0; j < 4; ++j) {
@@ -190,7 +194,7 @@ template <int DP, bool EXACT, int NW> __global__ __launch_bounds__(64 * NW) void
     __shared__ __attribute__((aligned(16))) float lds[64 * (DP + 4)];
     const int tid = threadIdx.x, lane = tid & 63, wave = tid >> 6, g = lane >> 4, col = lane & 15;
     const int M = p.Tq * p.G, Hq = p.Hk * p.G, tiles = (M + 15) / 16;
-    const int lin = on_xcd(blockIdx.x, tiles * p.B * p.Hk * p.nsplit), split = lin % p.nsplit;
+    const int lin = on_xcd(p, blockIdx.x, tiles * p.B * p.Hk * p.nsplit), split = lin % p.nsplit;
     const Where w = where(p, lin / p.nsplit, tiles);
     const int row0 = w.tile * 16, r = row0 + col, t = row_time(p, r), h = w.hk * p.G + r - t * p.G;
     const bool row = r < M && t < w.qlen;
@@ -205,6 +209,7 @@ template <int DP, bool EXACT, int NW> __global__ __launch_bounds__(64 * NW) void
         rows16<DP, EXACT>(f, base + (int64_t)min(key0 + col, kend - 1) * stride, p.D, g);
     };
     int key0 = kbeg + wave * 16;
+    uint8_t byte = key_byte(p, w, key0, kend, lane);
     if (key0 < kend) {
         fetch(x, k, p.ks[1], key0);
         fetch(y, v, p.vs[1], key0);
@@ -235,7 +240,7 @@ template <int DP, bool EXACT, int NW> __global__ __launch_bounds__(64 * NW) void
 #pragma unroll
     for (int s = 0; s < DP / 16; ++s) dQ[s] = f32x4{};
     for (; key0 < kend; key0 += 16 * NW) {
-        const uint32_t bits = (uint32_t)key_bits(p, w, key0, kend, lane) & 0xffffu;
+        const uint32_t bits = (uint32_t)key_bits(byte, key0, kend, lane) & 0xffffu;
         f32x4 S = {}, dP = {};
         edge16<DP, EXACT>(x, p.D, g);
 #pragma unroll
@@ -247,7 +252,10 @@ template <int DP, bool EXACT, int NW> __global__ __launch_bounds__(64 * NW) void
         edge16<DP, EXACT>(y, p.D, g);
 #pragma unroll
         for (int s = 0; s < DP / 16; ++s) dP = mma16(y[s], shared16<DP>(to, s, col, g), dP);
-        if (key0 + 16 * NW < kend) fetch(y, v, p.vs[1], key0 + 16 * NW);
+        if (key0 + 16 * NW < kend) {
+            byte = key_byte(p, w, key0 + 16 * NW, kend, lane);
+            fetch(y, v, p.vs[1], key0 + 16 * NW);
+        }
 #pragma unroll
         for (int j = 0; j < 4; ++j) S[j] = (bits >> (4 * g + j)) & 1 ? exp2_(fmaf(S[j], c, -lse2)) * (dP[j] - delta) : 0.f;
         if (bits != 0xffffu) keep16(x, bits, g);
@@ -270,10 +278,10 @@ template <int DP, bool EXACT, int NW> __global__ __launch_bounds__(64 * NW) void
     __shared__ __attribute__((aligned(16))) float lds[64 * (DP + 4)];
     const int tid = threadIdx.x, lane = tid & 63, wave = tid >> 6, g = lane >> 4, col = lane & 15;
     const int Hq = p.Hk * p.G, tiles = (p.Tk + 15) / 16;
-    const int lin = on_xcd(blockIdx.x, tiles * p.B * p.Hk * p.nsplit), split = lin % p.nsplit;
+    const int lin = on_xcd(p, blockIdx.x, tiles * p.B * p.Hk * p.nsplit), split = lin % p.nsplit;
     const Where w = where(p, lin / p.nsplit, tiles);
     const int key0 = w.tile * 16;
-    const uint32_t keys = (uint32_t)key_bits(p, w, key0, w.klen, lane) & 0xffffu;
+    const uint32_t keys = (uint32_t)key_bits(key_byte(p, w, key0, w.klen, lane), key0, w.klen, lane) & 0xffffu;
     const float c = p.scale * LOG2E;
     const int rows = keys ? w.qlen * p.G : 0;
     const int per = ((rows + 15) / 16 + p.nsplit - 1) / p.nsplit * 16;

@@ -29,7 +29,7 @@ __global__ __launch_bounds__(512) void attn_few(const AttnP p) {
     __shared__ float ml[NW][ROWS][2];
     const int tid = threadIdx.x, lane = tid & 63, wave = tid >> 6, group = lane >> 3, li = lane & 7;
     const int M = p.Tq * p.G;
-    const int lin = on_xcd(blockIdx.x, p.B * p.Hk * p.nsplit), split = lin % p.nsplit;
+    const int lin = on_xcd(p, blockIdx.x, p.B * p.Hk * p.nsplit), split = lin % p.nsplit;
     const Where w = where(p, lin / p.nsplit, 1);
     const float c = p.scale * LOG2E;
     const int per = ((w.klen + 7) / 8 + p.nsplit - 1) / p.nsplit * 8;

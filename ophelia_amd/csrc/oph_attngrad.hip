@@ -29,11 +29,41 @@ __global__ __launch_bounds__(256, (grad_waves<T, DP>(3))) void attn_dq(const Att
     __shared__ __attribute__((aligned(16))) char lds[4 * TB];
     const int tid = threadIdx.x, lane = tid & 63, wave = tid >> 6, half = lane >> 5, col = lane & 31;
     const int M = p.Tq * p.G, Hq = p.Hk * p.G, tiles = (M + 127) / 128;
-    const int lin = on_xcd(blockIdx.x, tiles * p.B * p.Hk * p.nsplit), split = lin % p.nsplit;
+    const int lin = on_xcd(p, blockIdx.x, tiles * p.B * p.Hk * p.nsplit), split = lin % p.nsplit;
     const Where w = where(p, lin / p.nsplit, tiles);
     const int r = w.tile * 128 + wave * 32 + col, t = row_time(p, r), h = w.hk * p.G + r - t * p.G;
     const bool row = r < M && t < w.qlen;
     const float c = p.scale * LOG2E;
+
+    const T* k = (const T*)p.k + w.b * p.ks[0] + w.hk * p.ks[2];
+    const T* v = (const T*)p.v + w.b * p.vs[0] + w.hk * p.vs[2];
+    const int per = ((w.klen + KT - 1) / KT + p.nsplit - 1) / p.nsplit * KT;
+    const int kbeg = split * per, kend = row_time(p, w.tile * 128) < w.qlen ? min(w.klen, kbeg + per) : kbeg;
+    const int nt = kend > kbeg ? (kend - kbeg + KT - 1) / KT : 0;
+    Stage<T, DP, KT, 256> sk, sv;
+    const T *k1 = sk.own(k + kbeg * p.ks[1], p.ks[1], p.D, tid), *v1 = sv.own(v + kbeg * p.vs[1], p.vs[1], p.D, tid);
+    uint64_t bits = 0;
+    uint8_t byte = 0;
+    auto fetch = [&](int j) {
+        const int key0 = kbeg + j * KT, last = kend - 1;
+        byte = key_byte(p, w, key0, kend, lane);
+        if (key0 + KT <= kend) {
+            sk.load_run(k1, p.ks[1]);
+            sv.load_run(v1, p.vs[1]);
+            k1 += KT * p.ks[1];
+            v1 += KT * p.vs[1];
+            return;
+        }
+        sk.load([&](int i) { return k + (int64_t)min(key0 + i, last) * p.ks[1]; }, p.D, tid);
+        sv.load([&](int i) { return v + (int64_t)min(key0 + i, last) * p.vs[1]; }, p.D, tid);
+    };
+    auto commit = [&](int j) {
+        char* x = lds + (j & 1) * 2 * TB;
+        bits = key_bits(byte, kbeg + j * KT, kend, lane) & FULL;
+        sk.store(x, bits, p.D, tid);
+        sv.store(x + TB, bits, p.D, tid);
+    };
+    if (nt) fetch(0);                                    // on its way while the rows' operands are loaded
 
     frag_t<T> Q[DP / 16], dO[DP / 16];
     f32x16 dQ[DP / 32];
@@ -61,34 +91,7 @@ __global__ __launch_bounds__(256, (grad_waves<T, DP>(3))) void attn_dq(const Att
 #pragma unroll
     for (int d = 0; d < DP / 32; ++d) dQ[d] = f32x16{};
 
-    const T* k = (const T*)p.k + w.b * p.ks[0] + w.hk * p.ks[2];
-    const T* v = (const T*)p.v + w.b * p.vs[0] + w.hk * p.vs[2];
-    const int per = ((w.klen + KT - 1) / KT + p.nsplit - 1) / p.nsplit * KT;
-    const int kbeg = split * per, kend = row_time(p, w.tile * 128) < w.qlen ? min(w.klen, kbeg + per) : kbeg;
-    const int nt = kend > kbeg ? (kend - kbeg + KT - 1) / KT : 0;
-    Stage<T, DP, KT, 256> sk, sv;
-    const T *k1 = sk.own(k + kbeg * p.ks[1], p.ks[1], p.D, tid), *v1 = sv.own(v + kbeg * p.vs[1], p.vs[1], p.D, tid);
-    uint64_t bits = 0, next = 0;
-    auto fetch = [&](int j) {
-        const int key0 = kbeg + j * KT, last = kend - 1;
-        next = key_bits(p, w, key0, kend, lane) & FULL;
-        if (key0 + KT <= kend) {
-            sk.load_run(k1, p.ks[1]);
-            sv.load_run(v1, p.vs[1]);
-            k1 += KT * p.ks[1];
-            v1 += KT * p.vs[1];
-            return;
-        }
-        sk.load([&](int i) { return k + (int64_t)min(key0 + i, last) * p.ks[1]; }, p.D, tid);
-        sv.load([&](int i) { return v + (int64_t)min(key0 + i, last) * p.vs[1]; }, p.D, tid);
-    };
-    auto commit = [&](int j) {
-        char* x = lds + (j & 1) * 2 * TB;
-        sk.store(x, next, p.D, tid);
-        sv.store(x + TB, next, p.D, tid);
-        bits = next;
-    };
-    if (nt) { fetch(0); commit(0); }
+    if (nt) commit(0);
     for (int j = 0; j < nt; ++j) {
         const uint64_t now = bits;
         __syncthreads();
@@ -153,32 +156,15 @@ __global__ __launch_bounds__(256, (grad_waves<T, DP>(2))) void attn_dkv(const At
     __shared__ __attribute__((aligned(16))) float stat[2][2][RT];       // lse (units of log2) and delta of a tile's rows
     const int tid = threadIdx.x, lane = tid & 63, wave = tid >> 6, half = lane >> 5, col = lane & 31;
     const int Hq = p.Hk * p.G, tiles = (p.Tk + 127) / 128;
-    int lin = on_xcd(blockIdx.x, tiles * p.B * p.Hk * p.nsplit * (BOTH ? 1 : 2));
+    int lin = on_xcd(p, blockIdx.x, tiles * p.B * p.Hk * p.nsplit * (BOTH ? 1 : 2));
     const bool want_dk = !BOTH && (lin & 1);                              // !BOTH: this workgroup's job
     if (!BOTH) lin >>= 1;
     const int split = lin % p.nsplit;
     const Where w = where(p, lin / p.nsplit, tiles);
     const int key = w.tile * 128 + wave * 32 + col;
-    const bool ok = (key_bits(p, w, w.tile * 128 + wave * 32, w.klen, lane) >> col) & 1;
+    const int first = w.tile * 128 + wave * 32;
+    const bool ok = (key_bits(key_byte(p, w, first, w.klen, lane), first, w.klen, lane) >> col) & 1;
     const float c = p.scale * LOG2E;
-
-    frag_t<T> K[DP / 16], V[DP / 16];
-    f32x16 acc[NACC][DP / 32];                                            // dv first
-    const int64_t kk = min(key, p.Tk - 1);
-    row_frags<T, DP>(K, (const T*)p.k + w.b * p.ks[0] + w.hk * p.ks[2] + kk * p.ks[1], p.D, ok, half);
-    char* tv = lds + 4 * TB + wave * TV;
-    if (BOTH || want_dk) {
-        row_frags<T, DP>(V, (const T*)p.v + w.b * p.vs[0] + w.hk * p.vs[2] + kk * p.vs[1], p.D, ok, half);
-        if constexpr (VLDS) {
-#pragma unroll
-            for (int s = 0; s < DP / 16; ++s) *(frag_t<T>*)(tv + col * Tile<T, DP>::STRIDE + (s * 16 + half * 8) * 2) = V[s];
-            wave_lds_fence();
-        }
-    }
-#pragma unroll
-    for (int a = 0; a < NACC; ++a)
-#pragma unroll
-        for (int d = 0; d < DP / 32; ++d) acc[a][d] = f32x16{};
 
     const int rows = w.tile * 128 < w.klen ? w.qlen * p.G : 0;
     const int per = ((rows + RT - 1) / RT + p.nsplit - 1) / p.nsplit * RT;
@@ -226,7 +212,27 @@ __global__ __launch_bounds__(256, (grad_waves<T, DP>(2))) void attn_dkv(const At
         so.store(x + TB, bits, p.D, tid);
         if (tid < RT) { stat[j & 1][0][tid] = lse2; stat[j & 1][1][tid] = delta; }
     };
-    if (nt) { fetch(0); commit(0); }
+    if (nt) fetch(0);                                    // on its way while the keys' operands are loaded
+
+    frag_t<T> K[DP / 16], V[DP / 16];
+    f32x16 acc[NACC][DP / 32];                                            // dv first
+    const int64_t kk = min(key, p.Tk - 1);
+    row_frags<T, DP>(K, (const T*)p.k + w.b * p.ks[0] + w.hk * p.ks[2] + kk * p.ks[1], p.D, ok, half);
+    char* tv = lds + 4 * TB + wave * TV;
+    if (BOTH || want_dk) {
+        row_frags<T, DP>(V, (const T*)p.v + w.b * p.vs[0] + w.hk * p.vs[2] + kk * p.vs[1], p.D, ok, half);
+        if constexpr (VLDS) {
+#pragma unroll
+            for (int s = 0; s < DP / 16; ++s) *(frag_t<T>*)(tv + col * Tile<T, DP>::STRIDE + (s * 16 + half * 8) * 2) = V[s];
+            wave_lds_fence();
+        }
+    }
+#pragma unroll
+    for (int a = 0; a < NACC; ++a)
+#pragma unroll
+        for (int d = 0; d < DP / 32; ++d) acc[a][d] = f32x16{};
+
+    if (nt) commit(0);
     for (int j = 0; j < nt; ++j) {
         __syncthreads();
         if (j + 1 < nt) fetch(j + 1);
@@ -347,6 +353,7 @@ template <class T, int DP> static int gradient(const oph_seq_attn* a, AttnP p, v
         p.nsplit = g.dq_split;
         p.o0 = a->dq;
         const int64_t groups = g.dq_units * g.dq_split;
+        p.chunk = run_of(a, groups, false);
         int rc;
         if constexpr (sizeof(T) == 4 && DP > 128) rc = attn16_launch(p, groups, 1, stream);
         else rc = g.small ? attn16_launch(p, groups, 1, stream) : launch<AttnP>(attn_dq<T, DP>, dim3((unsigned)groups), 256, p, 0, stream);
@@ -360,6 +367,7 @@ template <class T, int DP> static int gradient(const oph_seq_attn* a, AttnP p, v
         p.o0 = a->dv;
         p.o1 = a->dk;
         const int64_t groups = g.kv_units * g.kv_split;
+        p.chunk = run_of(a, groups, false);
         int rc;
         if constexpr (sizeof(T) == 4 && DP > 128) rc = attn16_launch(p, groups, 2, stream);
         else rc = g.small ? attn16_launch(p, groups, 2, stream) : launch<AttnP>(attn_dkv<T, DP, DP <= 128>, dim3((unsigned)groups), 256, p, 0, stream);
