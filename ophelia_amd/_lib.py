@@ -177,18 +177,20 @@ def libpath():
     return os.path.join(LIBDIR, "libophelia_hip.%s.so" % hashlib.md5(" ".join(more).encode()).hexdigest()[:8])
 
 
-def _hipcc_shared(out, srcs, deps, extra, verbose):
+def _hipcc_shared(out, srcs, deps, extra, verbose, force=False):
     # OPH_HIPCC_FLAGS: extra compiler flags (measurement builds); they go into a file of their own (libpath())
     more = os.environ.get("OPH_HIPCC_FLAGS", "").split() if os.path.basename(out).startswith("libophelia_hip") else []
-    if os.path.exists(out) and all(os.path.getmtime(out) >= os.path.getmtime(d) for d in deps):
+    if not force and os.path.exists(out) and all(os.path.getmtime(out) >= os.path.getmtime(d) for d in deps):
         return out
     extra = list(extra) + more
     hipcc = os.environ.get("HIPCC", "/opt/rocm/bin/hipcc")
     # several ranks may find the library stale at the same time: each builds into its own temporary file and renames
     # it into place (atomic on one filesystem), so a reader never maps a half-written library
     tmp = "%s.%d.tmp" % (out, os.getpid())
-    cmd = [hipcc, "--offload-arch=gfx950", "-O3", "-std=c++17", "-fPIC", "-shared",
-           "-Wno-unused-value", "-Wno-unused-result"] + srcs + extra + ["-o", tmp]
+    # packed fp32 instructions stay off: some of their forms have given wrong results on this hardware (the host pass does not know
+    # the feature and says so)
+    cmd = [hipcc, "--offload-arch=gfx950", "-O3", "-std=c++17", "-fPIC", "-shared", "-parallel-jobs=8",
+           "-Wno-unused-value", "-Wno-unused-result", "-Xclang", "-target-feature", "-Xclang", "-packed-fp32-ops"] + srcs + extra + ["-o", tmp]
     res = subprocess.run(cmd, stdout=subprocess.PIPE, stderr=subprocess.STDOUT, text=True)
     if verbose or res.returncode != 0:
         print(res.stdout)
@@ -200,21 +202,21 @@ def _hipcc_shared(out, srcs, deps, extra, verbose):
     return out
 
 
-def build(verbose=False):
-    """Compile the HIP extensions for gfx950 in-tree (cross-compiles without a GPU)."""
+def build(verbose=False, force=False):
+    """Compile the HIP extensions for gfx950 in-tree (cross-compiles without a GPU).  force: also those whose library is newer than its
+    sources."""
     os.makedirs(LIBDIR, exist_ok=True)
     inc = os.path.join(os.path.dirname(HERE), "include")
     srcs = [os.path.join(CSRC, s) for s in SOURCES]
     hdrs = [os.path.join(CSRC, "oph_internal.h"), os.path.join(CSRC, "oph_device.h"), os.path.join(CSRC, "oph_loopdev.h"), os.path.join(CSRC, "oph_host.h"),
             os.path.join(inc, "ophelia_hip.h")]
-    _hipcc_shared(libpath(), srcs, srcs + hdrs, ["-fvisibility=hidden"], verbose)
+    _hipcc_shared(libpath(), srcs, srcs + hdrs, ["-fvisibility=hidden"], verbose, force)
     vsrcs = [os.path.join(CSRC, s) for s in VOCODER_SOURCES]
     _hipcc_shared(VOCODER_LIBPATH, vsrcs, vsrcs + [os.path.join(inc, "ophelia_vocoder.h")],
-                  ["-L/opt/rocm/lib", "-lhipfft", "-Wl,-rpath,/opt/rocm/lib"], verbose)
-    # packed fp32 instructions stay off: some of their forms have given wrong results on this hardware
+                  ["-L/opt/rocm/lib", "-lhipfft", "-Wl,-rpath,/opt/rocm/lib"], verbose, force)
     ssrcs = [os.path.join(CSRC, s) for s in SEQ_SOURCES]
     _hipcc_shared(SEQ_LIBPATH, ssrcs, ssrcs + [os.path.join(CSRC, h) for h in SEQ_HEADERS] + [os.path.join(inc, "ophelia_seq.h"), os.path.join(inc, "ophelia_hip.h")],
-                  ["-fvisibility=hidden", "-Xclang", "-target-feature", "-Xclang", "-packed-fp32-ops"], verbose)
+                  ["-fvisibility=hidden"], verbose, force)
     return libpath()
 
 
