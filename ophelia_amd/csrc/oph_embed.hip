@@ -349,7 +349,7 @@ template <class T, class I> __global__ __launch_bounds__(256) void embed_rows(co
 static int check(const void* ids, int id_bytes, int64_t n, int64_t stride, int vocab, int units, float scale, int dtype, const char* what) {
     if (!type_bytes(dtype)) return fail(OPH_ERR_INVALID, "%s: dtype %d is not one of OPH_SEQ_*", what, dtype);
     if (id_bytes != 4 && id_bytes != 8) return fail(OPH_ERR_INVALID, "%s: ids of %d bytes (4 or 8)", what, id_bytes);
-    if (n < 0 || n > 1 << 28) return fail(OPH_ERR_INVALID, "%s: %lld ids", what, (long long)n);
+    if (n < 0 || n > 1 << 27) return fail(OPH_ERR_INVALID, "%s: %lld ids", what, (long long)n);
     if (vocab < 1 || vocab > 1 << 28 || units < 1 || units > 1 << 24) return fail(OPH_ERR_INVALID, "%s: table of %d rows of %d", what, vocab, units);
     if (stride < 0) return fail(OPH_ERR_INVALID, "%s: negative stride", what);
     if (n && !ids) return fail(OPH_ERR_INVALID, "%s: ids must not be NULL", what);

@@ -94,7 +94,7 @@ def test_attention(shape, dt):
 
 @dtypes
 @pytest.mark.parametrize("kind", ["ragged", "masked"])
-@pytest.mark.parametrize("shape", [(3, 1, 150, 2, 1, 256), (4, 40, 77, 4, 2, 64), (9, 129, 70, 32, 32, 48), (3, 5, 700, 4, 2, 128), (2, 300, 200, 2, 1, 96), (2, 70, 200, 3, 1, 200)], ids=str)
+@pytest.mark.parametrize("shape", [(5, 2, 90, 1, 1, 64), (4, 2, 300, 4, 2, 128), (3, 1, 150, 2, 1, 256), (4, 40, 77, 4, 2, 64), (9, 129, 70, 32, 32, 48), (3, 5, 700, 4, 2, 128), (2, 300, 200, 2, 1, 96), (2, 70, 200, 3, 1, 200)], ids=str)
 def test_attention_excluded_places_are_never_used(shape, kind, dt):
     _attend(shape, dt, kind, spoil=True)
 
@@ -283,6 +283,18 @@ def test_recurrence_gates_at_their_ends():
     gref, gb = O.recurrence_gradient(torch.ones(1, 600, 4), None, ctx)
     for n, a, r, b in zip(("dx", "dgate", "dh0"), M.gated_recurrence_gradient(torch.ones(1, 600, 4, device="cuda"), x.cuda(), g.cuda(), h, h0=h0.cuda()), gref, gb):
         _within(n, a, r, b)
+
+
+def test_recurrence_without_steps_hands_the_state_on():
+    from ophelia_amd import modules as M
+    for dt in DT:
+        x, h0 = torch.zeros(3, 0, 5, dtype=dt, device="cuda"), torch.randn(3, 5, device="cuda")
+        h, last = M.gated_recurrence(x, x, h0=h0)
+        assert h.shape == (3, 0, 5) and torch.equal(last, h0)
+        dx, dg, d0 = M.gated_recurrence_gradient(x, x, x, h, h0=h0, dh_last=h0)
+        assert dx.shape == dg.shape == (3, 0, 5) and torch.equal(d0, h0)
+        h, last = M.gated_recurrence(x[:0], x[:0])
+        assert h.shape == (0, 0, 5) and last.shape == (0, 5)
 
 
 def test_recurrence_steps_make_the_sequence():
