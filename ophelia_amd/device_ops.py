@@ -11,6 +11,7 @@ synchronise, so they can be captured into a graph.  Sums, statistics and states 
 which workgroups run.  Gradients are functions of their own: nothing here records for torch's autograd, and tensors that
 require gradients are refused outside torch.no_grad().  Bad arguments raise ValueError before anything is queued; there is
 no CPU fallback."""
+import operator
 import struct
 
 from . import _lib
@@ -115,8 +116,9 @@ def embed_gradient(ids, dout, vocab, scale=1.0, zero_pad=True):
     dout = _like(torch, "dout", dout, dtype, device, ids.shape + (U,))
     if dout.dim() != 2:
         dout = dout.reshape(-1, U)
-    if not isinstance(vocab, int) or vocab < 1:
-        raise ValueError("vocab must be a positive number of rows, is %r" % (vocab,))
+    vocab = operator.index(vocab)
+    if vocab < 1:
+        raise ValueError("vocab must be a positive number of rows, is %d" % vocab)
     lib, n = _lib.load_seq(), ids.numel()
     nbytes = _chk(lib.oph_seq_embed_workspace(n, vocab, U))
     ws = _workspace(torch, nbytes, device) if nbytes else None

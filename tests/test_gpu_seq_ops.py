@@ -223,8 +223,10 @@ def test_embed_all_tokens_alike_and_none():
     none = torch.zeros(2, 0, dtype=torch.int32, device="cuda")
     assert M.embed_lookup(none, torch.ones(4, 6, device="cuda")).shape == (2, 0, 6)
     assert not M.embed_gradient(none, torch.ones(2, 0, 6, device="cuda"), 4).any()
+    assert not M.embed_gradient(none, torch.ones(2, 0, 6, device="cuda"), 5000).any()
     pads = torch.zeros(50, dtype=torch.int32, device="cuda")                    # only padding, whatever its gradient holds
-    assert not M.embed_gradient(pads, torch.full((50, 6), math.nan, device="cuda"), 4).any()
+    for V in (4, 5000):
+        assert not M.embed_gradient(pads, torch.full((50, 6), math.nan, device="cuda"), V).any()
 
 
 def test_embed_strides_and_far_rows():
@@ -523,3 +525,32 @@ def test_synthesis_library_loaded_before_torch():
             "s.synchronize(); assert r.tolist() == [[6., 7., 8.], [3., 4., 5.]], r; print('right')")
     r = subprocess.run([sys.executable, "-c", code], cwd=ROOT, capture_output=True, text=True, timeout=100)
     assert r.returncode == 0 and "right" in r.stdout, (r.returncode, r.stdout[-500:], r.stderr[-1500:])
+
+
+def test_calls_on_two_streams_at_once():
+    """Long recurrences, whose blocks wait for one another inside a launch, and split attentions and embedding gradients, queued on two streams
+    without waiting: every result has the bits of the call alone."""
+    from ophelia_amd import modules as M
+    x = [_rand(s, (4, 6000, 192), torch.bfloat16).cuda() for s in (1, 2)]
+    g = [_rand(s, (4, 6000, 192), torch.bfloat16, 2.0).cuda() for s in (3, 4)]
+    q = [_rand(s, (2, 1, 8, 64), torch.bfloat16).cuda() for s in (5, 6)]
+    k = [_rand(s, (2, 5000, 2, 64), torch.bfloat16).cuda() for s in (7, 8)]
+    ids = [torch.randint(0, 3000, (9000,), generator=torch.Generator().manual_seed(s)).cuda() for s in (9, 10)]
+    d = [_rand(s, (9000, 64), torch.bfloat16).cuda() for s in (11, 12)]
+
+    def go(i):
+        h, last = M.gated_recurrence(x[i], g[i])
+        return [h, last, *M.gated_recurrence_gradient(x[i], x[i], g[i], h), *M.cross_attention(q[i], k[i], k[i]), M.embed_gradient(ids[i], d[i], 3000)]
+
+    want = [go(i) for i in (0, 1)]
+    torch.cuda.synchronize()
+    streams = [torch.cuda.Stream() for _ in (0, 1)]
+    got = [[], []]
+    for _ in range(6):
+        for i, s in enumerate(streams):
+            with torch.cuda.stream(s):
+                got[i].append(go(i))
+    torch.cuda.synchronize()
+    for i in (0, 1):
+        for r in got[i]:
+            assert all(torch.equal(a, b) for a, b in zip(r, want[i])), i
