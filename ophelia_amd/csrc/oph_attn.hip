@@ -365,8 +365,8 @@ static FwdPlan forward_plan(const oph_seq_attn* a) {
     // without matrix instructions: 16 x 1 row over 150 keys x 256 fp32 7.7 us (29 on 32-row products), 8 x 8 heads x 4 rows over 1000 keys x 128
     // bf16 15.0 (18.9); 4 rows of D <= 64 lose (8 x 8 heads over 4000 keys 25.7 and 20.6), 4 rows of D > 128 do not fit the registers
     f.few = M <= 2 || (M <= 4 && a->D > 64 && a->D <= 128);
-    // 128-row workgroups once they fill the CUs (fp32, 4 x 8 heads of 1024 x 1024 x 128: 163 us, 16-row units 240); below, units that
-    // split the keys (16 sequences of 200 x 150 x 256: 21 and 63)
+    // 128-row workgroups once they fill the CUs (fp32, 4 x 8 heads of 1024 x 1024 x 128: 158 us, 16-row units 254); below, units that
+    // split the keys (16 sequences of 200 x 150 x 256: 18 and 58)
     f.wide = !f.few && cdiv(M, 128) * heads >= 256;
     f.rows = a->dtype == OPH_SEQ_F32 ? unit_rows<float>() : unit_rows<f16_t>();
     f.units = cdiv(M, f.rows) * heads;

@@ -322,14 +322,16 @@ static int split_for(int64_t units, int64_t pieces, int64_t groups) {
 static GradPlan gradient_plan(const oph_seq_attn* a) {
     const int64_t M = (int64_t)a->Tq * (a->Hq / a->Hk), heads = (int64_t)a->B * a->Hk;
     GradPlan g;
-    // fp32 on 16x16 products: where 128 x 128 tiles are too few to fill the machine (16 sequences of 200 x 150 x 256: 75 us, 231 on the large
-    // tiles; 4 x 4 heads of 100 x 1500 x 64: 54 and 62), and for D > 128, where the large tiles' operands do not fit the registers (4 x 8 heads
-    // of 1024 x 1024 x 256: 2480 and 2817).  Elsewhere the shared tiles win (4 x 8 heads of 2048 x 256 x 64: 151 and 242).
-    g.small = a->dtype == OPH_SEQ_F32 && (a->D > 128 || cdiv(M, 128) * heads * cdiv(a->Tk, 128) * (a->D <= 64 ? 64 : 128) < 16384);
+    // fp32 on 16x16 products: where 128 x 128 tiles are too few to fill the machine and too few scores lie in them (16 sequences of 200 x 150:
+    // x 64 22 us, 63 on the large tiles, x 128 36 and 110; two heads of that x 128 70 and 111; but 4 x 4 heads of 100 x 1500 x 64 68 and 56,
+    // 64 x 8 heads of 30 x 30 x 64 34 and 28), and for D > 128, where the large tiles' operands do not fit the registers (4 x 8 heads of
+    // 1024 x 1024 x 256: 1490 and 2817).
+    g.small = a->dtype == OPH_SEQ_F32 &&
+              (a->D > 128 || (cdiv(M, 128) * heads * cdiv(a->Tk, 128) < 256 && M * heads * a->Tk < (a->D <= 64 ? 2300000 : 1600000)));
     const int rows = g.small ? 16 : 128, keys = g.small ? 16 : 128;
     g.dq_units = cdiv(M, rows) * heads;
     g.kv_units = cdiv(a->Tk, keys) * heads * (g.small || a->D <= 128 ? 1 : 2);
-    // one round of one or two workgroups a CU, at least 128 keys or rows a split (16 x 200 x 150 x 128 fp32: 37 us whole, 54 in two splits)
+    // one round of one or two workgroups a CU, at least 128 keys or rows a split (16 x 200 x 150 x 128 fp32: 36 us whole, 54 in two splits)
     const int64_t groups = a->D > 128 ? 256 : 512;
     g.dq_split = split_for(g.dq_units, a->Tk / 128, groups);
     g.kv_split = split_for(g.kv_units, M / 128, groups);

@@ -17,27 +17,29 @@ import struct
 from . import _lib
 
 _T = {}
-_state = {}
+_torch = None                 # the module, and below the library and the stream's raw handle: found at the first call
+_seq = None
+_stream = None
 # the argument structures of include/ophelia_seq.h as the compiler lays them out: packing them in one go is a third of the time that filling
 # ctypes fields takes, and a call on small tensors is bound by what happens here
 _ATTN = struct.Struct("@12P14qPN7if")
 _RECUR = struct.Struct("@11P8qPN4i")
-_NO_STRIDES = (0, 0, 0)
 
 
-def _torch():
+def _setup():
+    global _torch, _seq, _stream
     import torch
-    if not _T:
-        _T.update({torch.float32: _lib.SEQ_F32, torch.bfloat16: _lib.SEQ_BF16, torch.float16: _lib.SEQ_F16})
-        # the raw handle of the current stream without the stream object around it, where this torch has it
-        raw = getattr(torch._C, "_cuda_getCurrentRawStream", None)
-        _state["stream"] = raw or (lambda index: torch.cuda.current_stream(index).cuda_stream)
+    _T.update({torch.float32: _lib.SEQ_F32, torch.bfloat16: _lib.SEQ_BF16, torch.float16: _lib.SEQ_F16})
+    # the raw handle of the current stream without the stream object around it, where this torch has it
+    _stream = getattr(torch._C, "_cuda_getCurrentRawStream", None) or (lambda index: torch.cuda.current_stream(index).cuda_stream)
+    _seq = _lib.load_seq()
+    _torch = torch
     return torch
 
 
 def _chk(rc):
     if rc < 0:
-        raise _lib.OpheliaHipError("libophelia_seq error %d: %s" % (rc, _lib.load_seq().oph_seq_last_error().decode()))
+        raise _lib.OpheliaHipError("libophelia_seq error %d: %s" % (rc, _seq.oph_seq_last_error().decode()))
     return rc
 
 
@@ -52,13 +54,15 @@ def _first(torch, name, t):
 
 def _like(torch, name, t, dtype, device, shape):
     """A tensor of the call: type, device and shape as given, unit stride in the last axis."""
+    if isinstance(t, torch.Tensor) and t.dtype is dtype and t.shape == shape and t.device == device and not t.requires_grad:
+        return t if t.stride(-1) == 1 or t.shape[-1] == 1 else t.contiguous()
     if not isinstance(t, torch.Tensor) or t.dtype != dtype:
         raise ValueError("%s must be a %s tensor" % (name, dtype))
     if t.device != device:
         raise ValueError("%s is on %s, the call on %s" % (name, t.device, device))
     if t.shape != shape:
         raise ValueError("%s has shape %s, expected %s" % (name, tuple(t.shape), tuple(shape)))
-    if t.requires_grad and torch.is_grad_enabled():
+    if torch.is_grad_enabled():
         raise ValueError("%s requires a gradient: call under torch.no_grad() and use the gradient function" % name)
     return t if t.stride(-1) == 1 or t.shape[-1] == 1 else t.contiguous()
 
@@ -90,7 +94,7 @@ def _ids(torch, ids, device):
 def embed_lookup(ids, table, scale=1.0, zero_pad=True):
     """scale * table[ids]: ids of any shape, table (vocab, units) -> ids.shape + (units,).  zero_pad: id 0 reads as zeros, as
     everywhere in the reference (modules.py:38-40).  An id outside the table reads as zeros."""
-    torch = _torch()
+    torch = _torch or _setup()
     dtype, device = _first(torch, "table", table)
     if table.dim() != 2 or table.shape[0] < 1 or table.shape[1] < 1:
         raise ValueError("table must be (vocab, units), has shape %s" % (tuple(table.shape),))
@@ -98,8 +102,8 @@ def embed_lookup(ids, table, scale=1.0, zero_pad=True):
     ids, width = _ids(torch, ids, device)
     V, U = table.shape
     out = table.new_empty(ids.shape + (U,))
-    _chk(_lib.load_seq().oph_seq_embed_lookup(ids.data_ptr(), width, ids.numel(), table.data_ptr(), table.stride(0), V, U, float(scale),
-                                              bool(zero_pad), _T[dtype], out.data_ptr(), device.index, _state["stream"](device.index)))
+    _chk(_seq.oph_seq_embed_lookup(ids.data_ptr(), width, ids.numel(), table.data_ptr(), table.stride(0), V, U, float(scale),
+                                   bool(zero_pad), _T[dtype], out.data_ptr(), device.index, _stream(device.index)))
     return out
 
 
@@ -107,7 +111,7 @@ def embed_gradient(ids, dout, vocab, scale=1.0, zero_pad=True):
     """Gradient of embed_lookup with respect to its table: dout of shape ids.shape + (units,) -> (vocab, units) of dout's type, row v =
     scale * the sum of the dout rows whose id is v, taken in float32 in a fixed order.  Rows that no id names, and with zero_pad row 0, are
     zeros; ids outside the table are left out."""
-    torch = _torch()
+    torch = _torch or _setup()
     dtype, device = _first(torch, "dout", dout)
     ids, width = _ids(torch, ids, device)
     if dout.dim() < 1 or dout.shape[-1] < 1:
@@ -119,12 +123,12 @@ def embed_gradient(ids, dout, vocab, scale=1.0, zero_pad=True):
     vocab = operator.index(vocab)
     if vocab < 1:
         raise ValueError("vocab must be a positive number of rows, is %d" % vocab)
-    lib, n = _lib.load_seq(), ids.numel()
-    nbytes = _chk(lib.oph_seq_embed_workspace(n, vocab, U))
+    n = ids.numel()
+    nbytes = _chk(_seq.oph_seq_embed_workspace(n, vocab, U))
     ws = _workspace(torch, nbytes, device) if nbytes else None
     grad = dout.new_empty((vocab, U))
-    _chk(lib.oph_seq_embed_gradient(ids.data_ptr(), width, n, dout.data_ptr(), dout.stride(0), vocab, U, float(scale), bool(zero_pad),
-                                    _T[dtype], grad.data_ptr(), _ptr(ws), nbytes, device.index, _state["stream"](device.index)))
+    _chk(_seq.oph_seq_embed_gradient(ids.data_ptr(), width, n, dout.data_ptr(), dout.stride(0), vocab, U, float(scale), bool(zero_pad),
+                                     _T[dtype], grad.data_ptr(), _ptr(ws), nbytes, device.index, _stream(device.index)))
     return grad
 
 
@@ -143,25 +147,24 @@ def _recur(torch, x, gate, h0, lengths):
 
 def _run_recur(torch, call, gradient, pointers, strides, shape, dtype, device):
     """Fills the argument structure (include/ophelia_seq.h: oph_seq_recur), finds the workspace and makes the call."""
-    lib = _lib.load_seq()
     sizes = tuple(shape) + (_T[dtype],)
     a = _RECUR.pack(*pointers, *strides, 0, 0, *sizes)
-    nbytes = _chk(lib.oph_seq_recur_workspace(a, gradient))
+    nbytes = _chk(_seq.oph_seq_recur_workspace(a, gradient))
     if nbytes:
         ws = _workspace(torch, nbytes, device)
         a = _RECUR.pack(*pointers, *strides, ws.data_ptr(), nbytes, *sizes)
-    _chk(call(a, device.index, _state["stream"](device.index)))
+    _chk(call(a, device.index, _stream(device.index)))
 
 
 def gated_recurrence(x, gate, h0=None, lengths=None):
     """h_t = a_t h_{t-1} + (1 - a_t) x_t with a = sigmoid(gate): x, gate (B, T, C), h0 (B, C) float32 or None (zeros).  Returns h (B, T, C)
     of x's type and the state after the last step, (B, C) float32, which the next call takes as h0 (T = 1: one decoder step).
     lengths (B) int32: steps at or past a sequence's length are not read, keep its state and have h = 0."""
-    torch = _torch()
+    torch = _torch or _setup()
     dtype, device, shape, x, gate, h0, lens = _recur(torch, x, gate, h0, lengths)
     h = x.new_empty(shape)
     last = x.new_empty((shape[0], shape[2]), dtype=torch.float32)
-    _run_recur(torch, _lib.load_seq().oph_seq_recur_forward, 0,
+    _run_recur(torch, _seq.oph_seq_recur_forward, 0,
                (x.data_ptr(), gate.data_ptr(), _ptr(h0), h.data_ptr(), last.data_ptr(), 0, 0, 0, 0, 0, _ptr(lens)),
                x.stride()[:2] + gate.stride()[:2] + (0, 0, 0, 0), shape, dtype, device)
     return h, last
@@ -170,14 +173,14 @@ def gated_recurrence(x, gate, h0=None, lengths=None):
 def gated_recurrence_gradient(dh, x, gate, h, h0=None, dh_last=None, lengths=None):
     """Gradient of gated_recurrence: dh (B, T, C) and dh_last (B, C) float32 or None are the gradients of its two results, h its first
     result.  Returns dx, dgate (B, T, C), 0 past a sequence's length, and dh0 (B, C) float32 (dh_last for a sequence of length 0)."""
-    torch = _torch()
+    torch = _torch or _setup()
     dtype, device, shape, x, gate, h0, lens = _recur(torch, x, gate, h0, lengths)
     dh, h = _like(torch, "dh", dh, dtype, device, shape), _like(torch, "h", h, dtype, device, shape)
     state = (shape[0], shape[2])
     if dh_last is not None:
         dh_last = _like(torch, "dh_last", dh_last, torch.float32, device, state).contiguous()
     dx, dgate, dh0 = x.new_empty(shape), x.new_empty(shape), x.new_empty(state, dtype=torch.float32)
-    _run_recur(torch, _lib.load_seq().oph_seq_recur_gradient, 1,
+    _run_recur(torch, _seq.oph_seq_recur_gradient, 1,
                (x.data_ptr(), gate.data_ptr(), _ptr(h0), h.data_ptr(), 0, dh.data_ptr(), _ptr(dh_last), dx.data_ptr(), dgate.data_ptr(),
                 dh0.data_ptr(), _ptr(lens)),
                x.stride()[:2] + gate.stride()[:2] + h.stride()[:2] + dh.stride()[:2], shape, dtype, device)
@@ -206,13 +209,12 @@ def _attention(torch, q, k, v, q_lens, k_lens, key_mask, scale):
 
 def _run_attention(torch, call, gradient, pointers, strides, sizes, device):
     """Fills the argument structure (include/ophelia_seq.h: oph_seq_attn), finds the workspace and makes the call."""
-    lib = _lib.load_seq()
     a = _ATTN.pack(*pointers, *strides, 0, 0, *sizes)
-    nbytes = _chk(lib.oph_seq_attn_workspace(a, gradient))
+    nbytes = _chk(_seq.oph_seq_attn_workspace(a, gradient))
     if nbytes:
         ws = _workspace(torch, nbytes, device)
         a = _ATTN.pack(*pointers, *strides, ws.data_ptr(), nbytes, *sizes)
-    _chk(call(a, device.index, _state["stream"](device.index)))
+    _chk(call(a, device.index, _stream(device.index)))
 
 
 def cross_attention(q, k, v, q_lens=None, k_lens=None, key_mask=None, scale=None):
@@ -221,14 +223,14 @@ def cross_attention(q, k, v, q_lens=None, k_lens=None, key_mask=None, scale=None
     k_lens (B) int32 and key_mask (B, Tk) bool say which keys may be attended, q_lens (B) int32 which queries there are; what is
     excluded is never used, NaN included.  Returns out (B, Tq, Hq, D) and lse (B, Hq, Tq) float32, the logarithm of each row's sum of
     exponentials: exp(scale * q k^T - lse) are the alignments.  A row without key or query has out = 0 and lse = -inf."""
-    torch = _torch()
+    torch = _torch or _setup()
     dtype, device, q, k, v, ql, kl, sizes = _attention(torch, q, k, v, q_lens, k_lens, key_mask, scale)
     out = q.new_empty(q.shape)
     lse = q.new_empty((sizes[0], sizes[3], sizes[1]), dtype=torch.float32)
     mask = (0, 0) if key_mask is None else key_mask.stride()
-    _run_attention(torch, _lib.load_seq().oph_seq_attn_forward, 0,
+    _run_attention(torch, _seq.oph_seq_attn_forward, 0,
                    (q.data_ptr(), k.data_ptr(), v.data_ptr(), out.data_ptr(), lse.data_ptr(), 0, 0, 0, 0, _ptr(ql), _ptr(kl), _ptr(key_mask)),
-                   q.stride()[:3] + k.stride()[:3] + v.stride()[:3] + _NO_STRIDES + mask, sizes, device)
+                   q.stride()[:3] + k.stride()[:3] + v.stride()[:3] + (0, 0, 0) + mask, sizes, device)
     return out, lse
 
 
@@ -236,14 +238,14 @@ def cross_attention_gradient(dout, q, k, v, out, lse, q_lens=None, k_lens=None, 
     """Gradient of cross_attention: dout is the gradient of its first result, out and lse what it returned, the rest its arguments.
     Returns dq, dk, dv in the shapes of q, k, v, zero for queries and keys that took no part; k and v heads shared by several query
     heads get the sum over them, expanded (broadcast) inputs the gradient of every copy."""
-    torch = _torch()
+    torch = _torch or _setup()
     dtype, device, q, k, v, ql, kl, sizes = _attention(torch, q, k, v, q_lens, k_lens, key_mask, scale)
     dout = _like(torch, "dout", dout, dtype, device, q.shape)
     out = _like(torch, "out", out, dtype, device, q.shape).contiguous()
     lse = _like(torch, "lse", lse, torch.float32, device, (sizes[0], sizes[3], sizes[1])).contiguous()
     dq, dk, dv = q.new_empty(q.shape), q.new_empty(k.shape), q.new_empty(k.shape)
     mask = (0, 0) if key_mask is None else key_mask.stride()
-    _run_attention(torch, _lib.load_seq().oph_seq_attn_gradient, 1,
+    _run_attention(torch, _seq.oph_seq_attn_gradient, 1,
                    (q.data_ptr(), k.data_ptr(), v.data_ptr(), out.data_ptr(), lse.data_ptr(), dout.data_ptr(), dq.data_ptr(), dk.data_ptr(),
                     dv.data_ptr(), _ptr(ql), _ptr(kl), _ptr(key_mask)),
                    q.stride()[:3] + k.stride()[:3] + v.stride()[:3] + dout.stride()[:3] + mask, sizes, device)
