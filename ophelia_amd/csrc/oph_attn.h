@@ -10,6 +10,7 @@
 // order: element j of lane half e is row 16s + 8(j/4) + 4e + j%4.  trans_frag() reads them so from a row-major tile in LDS.
 #pragma once
 #include "oph_seq.h"
+#include "oph_split.h"
 
 #pragma GCC visibility push(hidden)
 namespace ophseq {
@@ -62,9 +63,10 @@ __device__ __forceinline__ const T* row_ptr(const AttnP& p, const void* base, co
 }
 
 // Which of the keys key0 + lane may be attended, in two steps: the mask's byte is loaded with (before) the keys it belongs to, and only
-// asked for when they are used.  bit i of key_bits(): key key0 + i (i < 64).
+// asked for when they are used.  Nothing is read where no key before kend is left.  bit i of key_bits(): key key0 + i (i < 64).
 __device__ __forceinline__ uint8_t key_byte(const AttnP& p, const Where& w, int key0, int kend, int lane) {
-    return p.mask && kend > 0 ? p.mask[w.b * p.ms[0] + min(key0 + lane, kend - 1) * p.ms[1]] : 1;
+    const int at = flag_index(key0, lane, kend);
+    return p.mask && at >= 0 ? p.mask[w.b * p.ms[0] + at * p.ms[1]] : 1;
 }
 __device__ __forceinline__ uint64_t key_bits(uint8_t byte, int key0, int kend, int lane) { return __ballot(byte != 0 && key0 + lane < kend); }
 

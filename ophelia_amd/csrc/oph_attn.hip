@@ -182,8 +182,8 @@ __global__ __launch_bounds__(256) void attn_split(const AttnP p) {
     const Where w = where(p, lin / p.nsplit, tiles);
     const int row0 = w.tile * 32;
     const float c = p.scale * LOG2E;
-    const int per = ((w.klen + 31) / 32 + p.nsplit - 1) / p.nsplit * 32;
-    const int kbeg = split * per, kend = row_time(p, row0) < w.qlen ? min(w.klen, kbeg + per) : kbeg;
+    const Span span = split_span(w.klen, 32, p.nsplit, split, row_time(p, row0) < w.qlen);
+    const int kbeg = span.beg, kend = span.end;
 
     frag_t<T> Q[DP / 16];
     f32x16 O[DP / 32];

@@ -108,8 +108,8 @@ template <int DP, bool EXACT, int NW> __global__ __launch_bounds__(64 * NW) void
     const Where w = where(p, lin / p.nsplit, tiles);
     const int row0 = w.tile * 16;
     const float c = p.scale * LOG2E;
-    const int per = ((w.klen + 15) / 16 + p.nsplit - 1) / p.nsplit * 16;
-    const int kbeg = split * per, kend = row_time(p, row0) < w.qlen ? min(w.klen, kbeg + per) : kbeg;
+    const Span span = split_span(w.klen, 16, p.nsplit, split, row_time(p, row0) < w.qlen);
+    const int kbeg = span.beg, kend = span.end;
     const float* k = (const float*)p.k + w.b * p.ks[0] + w.hk * p.ks[2];
     const float* v = (const float*)p.v + w.b * p.vs[0] + w.hk * p.vs[2];
     f32x4 O[DP / 16], x[DP / 16], y[DP / 16];                            // x: rows of keys, y: columns of values
@@ -201,8 +201,8 @@ template <int DP, bool EXACT, int NW> __global__ __launch_bounds__(64 * NW) void
     const int row0 = w.tile * 16, r = row0 + col, t = row_time(p, r), h = w.hk * p.G + r - t * p.G;
     const bool row = r < M && t < w.qlen;
     const float c = p.scale * LOG2E;
-    const int per = ((w.klen + 15) / 16 + p.nsplit - 1) / p.nsplit * 16;
-    const int kbeg = split * per, kend = row_time(p, row0) < w.qlen ? min(w.klen, kbeg + per) : kbeg;
+    const Span span = split_span(w.klen, 16, p.nsplit, split, row_time(p, row0) < w.qlen);
+    const int kbeg = span.beg, kend = span.end;
     const float* k = (const float*)p.k + w.b * p.ks[0] + w.hk * p.ks[2];
     const float* v = (const float*)p.v + w.b * p.vs[0] + w.hk * p.vs[2];
     f32x4 dQ[DP / 16], x[DP / 16], y[DP / 16];                           // x: rows, then columns of keys, y: rows of values
@@ -286,8 +286,8 @@ template <int DP, bool EXACT, int NW> __global__ __launch_bounds__(64 * NW) void
     const uint32_t keys = (uint32_t)key_bits(key_byte(p, w, key0, w.klen, lane), key0, w.klen, lane) & 0xffffu;
     const float c = p.scale * LOG2E;
     const int rows = keys ? w.qlen * p.G : 0;
-    const int per = ((rows + 15) / 16 + p.nsplit - 1) / p.nsplit * 16;
-    const int rbeg = split * per, rend = min(rows, rbeg + per);
+    const Span span = split_span(rows, 16, p.nsplit, split, true);
+    const int rbeg = span.beg, rend = span.end;
     f32x4 dK[DP / 16], dV[DP / 16], x[DP / 16], y[DP / 16];              // x: rows of q, columns of dout, y: rows of dout, columns of q
     float *tk = lds, *tv = lds + 16 * (DP + 4);
     auto q_row = [&](int r) { return row_ptr<float>(p, p.q, w, min(r, rend - 1), p.qs[0], p.qs[1], p.qs[2]); };

@@ -32,8 +32,8 @@ __global__ __launch_bounds__(512) void attn_few(const AttnP p) {
     const int lin = on_xcd(p, blockIdx.x, p.B * p.Hk * p.nsplit), split = lin % p.nsplit;
     const Where w = where(p, lin / p.nsplit, 1);
     const float c = p.scale * LOG2E;
-    const int per = ((w.klen + 7) / 8 + p.nsplit - 1) / p.nsplit * 8;
-    const int kbeg = split * per, kend = w.qlen > 0 ? min(w.klen, kbeg + per) : kbeg;
+    const Span span = split_span(w.klen, 8, p.nsplit, split, w.qlen > 0);
+    const int kbeg = span.beg, kend = span.end;
 
     float q[ROWS][E], acc[ROWS][E], m[ROWS], l[ROWS];
 #pragma unroll

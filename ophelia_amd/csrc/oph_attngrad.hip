@@ -37,8 +37,8 @@ __global__ __launch_bounds__(256, (grad_waves<T, DP>(3))) void attn_dq(const Att
 
     const T* k = (const T*)p.k + w.b * p.ks[0] + w.hk * p.ks[2];
     const T* v = (const T*)p.v + w.b * p.vs[0] + w.hk * p.vs[2];
-    const int per = ((w.klen + KT - 1) / KT + p.nsplit - 1) / p.nsplit * KT;
-    const int kbeg = split * per, kend = row_time(p, w.tile * 128) < w.qlen ? min(w.klen, kbeg + per) : kbeg;
+    const Span span = split_span(w.klen, KT, p.nsplit, split, row_time(p, w.tile * 128) < w.qlen);
+    const int kbeg = span.beg, kend = span.end;
     const int nt = kend > kbeg ? (kend - kbeg + KT - 1) / KT : 0;
     Stage<T, DP, KT, 256> sk, sv;
     const T *k1 = sk.own(k + kbeg * p.ks[1], p.ks[1], p.D, tid), *v1 = sv.own(v + kbeg * p.vs[1], p.vs[1], p.D, tid);
@@ -167,8 +167,8 @@ __global__ __launch_bounds__(256, (grad_waves<T, DP>(2))) void attn_dkv(const At
     const float c = p.scale * LOG2E;
 
     const int rows = w.tile * 128 < w.klen ? w.qlen * p.G : 0;
-    const int per = ((rows + RT - 1) / RT + p.nsplit - 1) / p.nsplit * RT;
-    const int rbeg = split * per, rend = min(rows, rbeg + per);
+    const Span span = split_span(rows, RT, p.nsplit, split, true);
+    const int rbeg = span.beg, rend = span.end;
     const int nt = rend > rbeg ? (rend - rbeg + RT - 1) / RT : 0;
     Stage<T, DP, RT, 256> sq, so;
     float lse2 = INFINITY, delta = 0.f;

@@ -554,3 +554,26 @@ def test_calls_on_two_streams_at_once():
     for i in (0, 1):
         for r in got[i]:
             assert all(torch.equal(a, b) for a, b in zip(r, want[i])), i
+
+
+@dtypes
+@pytest.mark.parametrize("D", [64, 72, 128, 256])
+def test_attention_padded_rows_of_split_masked_keys(D, dt):
+    """A mask, and lengths that leave whole tiles of rows without a query, where the keys are split so often that the last pieces begin
+    behind the keys: a padded tile reads no key and no byte of the mask."""
+    from ophelia_amd import modules as M
+    B, Tq, Tk = 2, 48, 2049
+    q, k, v, do = _case((B, Tq, Tk, 1, 1, D), dt, 31)
+    ql, kl = torch.tensor([16, 33], dtype=torch.int32), torch.tensor([Tk, 40], dtype=torch.int32)
+    mask = torch.rand(B, Tk, generator=torch.Generator().manual_seed(6)) < 0.7
+    out, lse, bo, bl, ctx = O.attention(q, k, v, ql, kl, mask)
+    ref, bound = O.attention_gradient(do, ctx)
+    qd, kd, vd, dd, qld, kld = _cuda(q, k, v, do, ql, kl)
+    wide = torch.zeros(B, 2 * Tk, dtype=torch.bool, device="cuda")
+    wide[:, ::2] = mask.cuda()
+    for m in (mask.cuda(), wide[:, ::2]):                                  # every byte, and every other one
+        o, l = M.cross_attention(qd, kd, vd, q_lens=qld, k_lens=kld, key_mask=m)
+        _within("out", o, out, bo)
+        _within("lse", l, lse, bl)
+        for n, g, r, b in zip(("dq", "dk", "dv"), M.cross_attention_gradient(dd, qd, kd, vd, o, l, q_lens=qld, k_lens=kld, key_mask=m), ref, bound):
+            _within(n, g, r, b)

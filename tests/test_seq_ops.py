@@ -3,6 +3,7 @@ fails loudly where there is none."""
 import ctypes as C
 import os
 import re
+import subprocess
 
 import pytest
 import torch
@@ -128,3 +129,51 @@ def test_packed_arguments_match_the_structures():
     assert (a.workspace, a.workspace_bytes, a.B, a.Hk, a.dtype, a.scale) == (200, 201, 300, 304, 306, 0.5)
     r = _lib.OphSeqRecur.from_buffer_copy(device_ops._RECUR.pack(*range(11), *range(100, 108), 200, 201, *range(300, 304)))
     assert (r.gate, r.lens, list(r.dh_stride), r.workspace, r.workspace_bytes, r.B, r.dtype) == (1, 10, [106, 107], 200, 201, 300, 303)
+
+
+def test_split_spans_stay_inside_their_axis(tmp_path):
+    """The spans of a split axis and the places their flags are read from (csrc/oph_split.h), compiled for the CPU: in order, whole, inside the
+    axis, also where the rounded-up pieces of a padded tile begin behind it and where the last one's end passes 32 bits."""
+    src = tmp_path / "spans.cpp"
+    src.write_text(r'''
+#include "oph_split.h"
+#include <cstdio>
+#include <initializer_list>
+using namespace ophseq;
+static long bad = 0, seen = 0;
+static void look(int n, int tile, int nsplit) {
+    int at = 0;
+    for (int s = 0; s < nsplit; ++s)
+        for (int live = 0; live < 2; ++live) {
+            const Span x = split_span(n, tile, nsplit, s, live);
+            bad += x.beg < 0 || x.beg > x.end || x.end > n || (!live && x.end != x.beg);
+            if (live) { bad += x.beg != at || (x.beg < n && x.beg % tile); at = x.end; }
+            for (int wave = 0; wave < 8; ++wave)                     // a wave's first tile, there or not
+                for (int lane = 0; lane < 64; lane += 21) {
+                    const int i = flag_index(x.beg + wave * tile, lane, x.end), want = x.beg + wave * tile + lane;
+                    ++seen;
+                    bad += i >= n || i < -1 || (want < x.end && i != want) || (x.beg + wave * tile >= x.end && i != -1);
+                }
+        }
+    bad += at != n;
+}
+int main() {
+    const int tiles[] = {8, 16, 32, 64}, few[] = {0, 1, 7, 16, 17, 150, 2049, 8197, 32772};
+    for (int tile : tiles) {
+        for (int n = 0; n < 700; n += 1 + n / 40)
+            for (int ns = 1; ns <= 256; ns += 1 + ns / 8) look(n, tile, ns);
+        for (int n : few)
+            for (int ns = 1; ns <= 256; ++ns) look(n, tile, ns);
+        for (int n : {2147482743, 2147482000, 2147480000})
+            for (int ns : {1, 3, 16, 255, 256}) look(n, tile, ns);
+    }
+    std::printf("%ld looked at, %ld bad\n", seen, bad);
+    return bad != 0;
+}
+''')
+    exe = str(tmp_path / "spans")
+    # signed overflow ends the program: a sum that leaves 32 bits is found even where the result happens to look right
+    subprocess.run(["g++", "-std=c++17", "-O1", "-fsanitize=undefined", "-fno-sanitize-recover=undefined", "-I", os.path.join(ROOT, "ophelia_amd", "csrc"),
+                    str(src), "-o", exe], check=True, timeout=120)
+    r = subprocess.run([exe], capture_output=True, text=True, timeout=120)
+    assert r.returncode == 0, (r.stdout[-500:], r.stderr[-1500:])
