@@ -79,6 +79,8 @@ int oph_seq_embed_gradient(const void* ids, int id_bytes, int64_t n, const void*
  * x, gate (B,T,C): a = sigmoid(gate), h_t = a_t h_{t-1} + (1 - a_t) x_t from h0 (B,C) float32 (NULL: 0); h (B,T,C) contiguous,
  * h_last (B,C) float32 = the state after the last step.  Steps t >= lens[b] (NULL: T) are not used, leave the state as it is, and
  * have h = 0 and gradients 0.  The gradient takes the forward's h; dh_last (NULL: 0), dh0 float32 (B,C); dx, dgate contiguous.
+ * Its states are float32: h itself in OPH_SEQ_F32; in 16 bits, where h is rounded, they are formed again from x, gate and h0, and h's values
+ * are not used.
  * h0 may be h_last's buffer (the state of a step-by-step decoder, updated in place). */
 typedef struct oph_seq_recur {
     const void *x, *gate;
@@ -91,10 +93,11 @@ typedef struct oph_seq_recur {
     float* dh0;
     const int32_t* lens;
     int64_t x_stride[2], gate_stride[2], h_stride[2], dh_stride[2];   /* of B, T */
-    void* workspace;
+    void* workspace;                 /* oph_seq_recur_workspace() bytes, 16-byte aligned; NULL if 0 */
     size_t workspace_bytes;
     int32_t B, T, C, dtype;
 } oph_seq_recur;
+/* bytes of workspace that a call with these sizes and dtype needs; gradient: 0 forward, 1 gradient.  Negative: oph_status. */
 int64_t oph_seq_recur_workspace(const oph_seq_recur* a, int gradient);
 int oph_seq_recur_forward(const oph_seq_recur* a, int device, void* stream);
 int oph_seq_recur_gradient(const oph_seq_recur* a, int device, void* stream);

@@ -14,6 +14,12 @@
 // canonical one), and words are written and read whole, past the caches that the XCDs do not share.
 //
 // Gradient, backwards in time with the map m_t = a_t (m_{t+1} + dh_t):  l_t = dh_t + m_{t+1}, dx = (1 - a) l, dgate = a (1 - a) (h_{t-1} - x) l.
+// h_{t-1} - x has to come from a float32 state: where the state follows its input the two are nearly the same, and the half step (2^-9 of h in
+// bfloat16) that the forward's result is rounded by would be all that is left of the difference.  In float32 the result is the state and
+// is read; in 16 bits the states are formed again: a sequence of one block does so from the x and gate that it holds in registers, and for longer
+// ones a pass of the forward's chain leaves the state before every stretch in the workspace, from which the stretch is run once more.  4 x
+// 16384 x 1024 bf16: 129 us that pass, 225 the gradient; 120 and 288 with the states behind the blocks only, since composing the
+// stretches again takes 250 registers; 200 in one pass from the rounded states, which cost dgate up to all of its digits.
 #include "oph_seq.h"
 #include "../../include/ophelia_hip.h"
 
@@ -31,12 +37,14 @@ struct RecurP {
     unsigned long long* map;                                           // [chain][block][channel] {A, B}
     unsigned* state;                                                   // [chain][block][channel] state behind the block
     unsigned* ticket;
+    float* stretch;                                                    // gradient in 16 bits: [chain][block][stretch][channel] state before it
     int B, T, C, blocks;
 };
 constexpr int R = 4, WINDOW = 16;                                      // steps of a stretch | maps taken at once
 // Waves of a workgroup, and with them the steps of a block (8 stretches a wave).  Up to 256 steps are one block of 8 waves, with
 // nothing to hand on (16 x 200 x 256 fp32: 6.9 us; as two blocks of 4 waves and the clearing launch 11.4).  Longer ones are
-// blocks of 4 waves: more of them wait for memory side by side (4 x 16384 x 1024 bf16, both directions: 326 us; 8 waves 360, 16 waves 404).
+// blocks of 4 waves: more of them wait for memory side by side (4 x 16384 x 1024 bf16, forward, and gradient in one pass: 326 us; 8 waves 360,
+// 16 waves 404).
 constexpr int ONE = 8, MANY = 4;
 constexpr int block_steps(int nw) { return nw * 8 * R; }
 
@@ -173,7 +181,8 @@ __device__ __forceinline__ float compose(const RecurP& p, float (&A)[PER], float
     return behind;
 }
 
-template <class T, int NW> __global__ __launch_bounds__(64 * NW) void recur_forward(const RecurP p) {
+// STATES: no results but the states before the stretches
+template <class T, int NW, bool STATES> __global__ __launch_bounds__(64 * NW) void recur_forward(const RecurP p) {
     constexpr int PER = El<T>::PER16, CH = 8 * PER, BLOCK = block_steps(NW);
     __shared__ Shared<PER, NW> sh;
     const int tid = threadIdx.x, sub = tid >> 3, slabs = (p.C + CH - 1) / CH;
@@ -186,6 +195,7 @@ template <class T, int NW> __global__ __launch_bounds__(64 * NW) void recur_forw
     const int t = at.y * BLOCK + sub * R;
     T* h = (T*)p.h + (int64_t)b * p.T * p.C + cc;
     const float zero[PER] = {};
+    if (STATES && at.y * BLOCK >= len) return;
     if (at.y * BLOCK >= len) {                                           // nothing to do here but zeros; block 0 hands the state on
         if (left > 0)
 #pragma unroll
@@ -221,6 +231,12 @@ template <class T, int NW> __global__ __launch_bounds__(64 * NW) void recur_forw
     }
     const bool last = (at.y + 1) * BLOCK >= len;
     const float behind = compose<PER, NW>(p, A, B, first, s, at.x, at.y, last, sh);
+    if (STATES) {
+        float* to = p.stretch + (((int64_t)at.x * p.blocks + at.y) * (NW * 8) + sub) * CH + c - c0;
+#pragma unroll
+        for (int j = 0; j < PER; j += 4) *(f32x4*)(to + j) = f32x4{s[j], s[j + 1], s[j + 2], s[j + 3]};
+        return;
+    }
     if (last && mine) p.h_last[one] = behind;
 #pragma unroll
     for (int r = 0; r < R; ++r) {
@@ -236,29 +252,77 @@ template <class T, int NW> __global__ __launch_bounds__(64 * NW) void recur_forw
     }
 }
 
-// block k holds the BLOCK steps that end k * BLOCK before the sequence's end, latest first
+// The state before this thread's steps t-R+1, ..., t of the only block -> s, which comes as the state before the block: the forward's operations,
+// with the later of two stretches in the lower lanes and waves.  All threads call it.
+template <class T, int NW>
+__device__ __forceinline__ void before_stretch(float (&s)[El<T>::PER16], const u32x4 (&xr)[R], const u32x4 (&gr)[R], int t, int len,
+                                               float (&maps)[NW][8 * El<T>::PER16][2]) {
+    constexpr int PER = El<T>::PER16;
+    const int lane = threadIdx.x & 63, wave = threadIdx.x >> 6, cg = (lane & 7) * PER;
+    float A[PER], B[PER];
+#pragma unroll
+    for (int j = 0; j < PER; ++j) {
+        A[j] = 1.f;
+        B[j] = 0.f;
+#pragma unroll
+        for (int r = R - 1; r >= 0; --r) {
+            float a, keep;
+            gate_of(Piece<T>::at(gr[r], j), a, keep);
+            if (t - r < len) {
+                A[j] *= a;
+                B[j] = fmaf(a, B[j], keep * Piece<T>::at(xr[r], j));
+            }
+        }
+    }
+#pragma unroll
+    for (int off = 8; off < 64; off <<= 1)
+#pragma unroll
+        for (int j = 0; j < PER; ++j) {
+            const float a = __shfl_down(A[j], off), b = __shfl_down(B[j], off);
+            if (lane + off < 64) {
+                B[j] = fmaf(A[j], b, B[j]);
+                A[j] *= a;
+            }
+        }
+    if (lane < 8)
+#pragma unroll
+        for (int j = 0; j < PER; ++j) { maps[wave][cg + j][0] = A[j]; maps[wave][cg + j][1] = B[j]; }
+    __syncthreads();
+#pragma unroll
+    for (int j = 0; j < PER; ++j) {
+        float pa = __shfl_down(A[j], 8), pb = __shfl_down(B[j], 8);
+        if (lane >= 56) { pa = 1.f; pb = 0.f; }
+        for (int w = NW - 1; w > wave; --w) s[j] = fmaf(maps[w][cg + j][0], s[j], maps[w][cg + j][1]);
+        s[j] = fmaf(pa, s[j], pb);
+    }
+}
+
+// the forward's blocks, latest first; those behind the sequence's end come after them
 template <class T, int NW> __global__ __launch_bounds__(64 * NW) void recur_gradient(const RecurP p) {
     constexpr int PER = El<T>::PER16, CH = 8 * PER, BLOCK = block_steps(NW);
+    constexpr bool AGAIN = sizeof(T) == 2;                               // the forward's result is not the state
     __shared__ Shared<PER, NW> sh;
+    __shared__ float maps[AGAIN && NW == ONE ? NW : 1][CH][2];
     const int tid = threadIdx.x, sub = tid >> 3, slabs = (p.C + CH - 1) / CH;
     const int2 at = place<PER, NW>(p, p.B * slabs, sh);
     const int b = at.x / slabs, c0 = (at.x - b * slabs) * CH, c = c0 + (tid & 7) * PER, left = p.C - c;
-    const int len = p.lens ? min(max(p.lens[b], 0), p.T) : p.T;
+    const int len = p.lens ? min(max(p.lens[b], 0), p.T) : p.T, blocks = (len + BLOCK - 1) / BLOCK;
     const int cc = left > 0 ? c : 0, cl = left > 0 ? left : p.C;
     const bool mine = tid < CH && c0 + tid < p.C;
     const int64_t one = (int64_t)b * p.C + c0 + tid;
+    const int block = at.y < blocks ? blocks - 1 - at.y : at.y;          // in time
+    const int t = block * BLOCK + BLOCK - 1 - sub * R;                   // this thread: t, t-1, ..., t-R+1
     T* dx = (T*)p.dx + (int64_t)b * p.T * p.C + cc;
     T* dg = (T*)p.dgate + (int64_t)b * p.T * p.C + cc;
     const float zero[PER] = {};
-    if ((at.y + 1) * BLOCK > len && left > 0)                            // zeros behind the end, by the place in time
-        for (int r = 0; r < R; ++r) {
-            const int z = at.y * BLOCK + sub * R + r;
-            if (z >= len && z < p.T) {
-                Piece<T>::store(dx + (int64_t)z * p.C, zero, left);
-                Piece<T>::store(dg + (int64_t)z * p.C, zero, left);
-            }
-        }
-    if (at.y * BLOCK >= len) {
+    if (at.y >= blocks) {
+        if (left > 0)
+#pragma unroll
+            for (int r = 0; r < R; ++r)
+                if (t - r < p.T) {
+                    Piece<T>::store(dx + (int64_t)(t - r) * p.C, zero, left);
+                    Piece<T>::store(dg + (int64_t)(t - r) * p.C, zero, left);
+                }
         if (at.y == 0 && mine && p.dh0) p.dh0[one] = p.dh_last ? p.dh_last[one] : 0.f;
         return;
     }
@@ -266,60 +330,80 @@ template <class T, int NW> __global__ __launch_bounds__(64 * NW) void recur_grad
     const T* g = (const T*)p.gate + b * p.gs[0] + cc;
     const T* h = (const T*)p.hin + b * p.hs[0] + cc;
     const T* d = (const T*)p.dh + b * p.ds[0] + cc;
-    const int t = len - 1 - at.y * BLOCK - sub * R;                      // this thread: t, t-1, ..., t-R+1
     u32x4 xr[R], gr[R], hr[R], dr[R];
 #pragma unroll
     for (int r = 0; r < R; ++r) {
-        const int64_t tt = max(t - r, 0);
+        const int64_t tt = min(t - r, len - 1);
         gr[r] = Piece<T>::load(g + tt * p.gs[1], cl);
         dr[r] = Piece<T>::load(d + tt * p.ds[1], cl);
         xr[r] = Piece<T>::load(x + tt * p.xs[1], cl);
-        hr[r] = Piece<T>::load(h + max(tt - 1, (int64_t)0) * p.hs[1], cl);
+        if (!AGAIN) hr[r] = Piece<T>::load(h + max(tt - 1, (int64_t)0) * p.hs[1], cl);
     }
     const float first = at.y == 0 && mine && p.dh_last ? p.dh_last[one] : 0.f;
-    float A[PER], B[PER], s[PER], h0[PER];
+    float A[PER], B[PER], s[PER], h0[PER];                               // h0: the state before step 0; 16 bits, later: before the stretch
 #pragma unroll
     for (int j = 0; j < PER; ++j) {
-        h0[j] = p.h0 && t - R < 0 && j < left ? p.h0[(int64_t)b * p.C + c + j] : 0.f;
+        h0[j] = p.h0 && block == 0 && j < left ? p.h0[(int64_t)b * p.C + c + j] : 0.f;
         A[j] = 1.f;
         B[j] = 0.f;
 #pragma unroll
         for (int r = 0; r < R; ++r) {
             float a, keep;
             gate_of(Piece<T>::at(gr[r], j), a, keep);
-            if (t - r >= 0) {
+            if (t - r < len) {
                 A[j] *= a;
                 B[j] = a * (B[j] + Piece<T>::at(dr[r], j));
             }
         }
     }
-    const bool last = (at.y + 1) * BLOCK >= len;
+    if (AGAIN && NW != ONE) {
+        const float* from = p.stretch + (((int64_t)at.x * p.blocks + block) * (NW * 8) + NW * 8 - 1 - sub) * CH + c - c0;
+#pragma unroll
+        for (int j = 0; j < PER; j += 4) {
+            const f32x4 v = *(const f32x4*)(from + j);
+            h0[j] = v[0]; h0[j + 1] = v[1]; h0[j + 2] = v[2]; h0[j + 3] = v[3];
+        }
+    }
+    const bool last = block == 0;
     const float behind = compose<PER, NW>(p, A, B, first, s, at.x, at.y, last, sh);
     if (last && mine && p.dh0) p.dh0[one] = behind;
+    if constexpr (AGAIN && NW == ONE) before_stretch<T, NW>(h0, xr, gr, t, len, maps);
+    float hb[R][PER];                                                    // h_{t-1} of the steps
+#pragma unroll
+    for (int r = R - 1; r >= 0; --r)
+#pragma unroll
+        for (int j = 0; j < PER; ++j) {
+            hb[r][j] = AGAIN || t - r == 0 ? h0[j] : Piece<T>::at(hr[r], j);
+            if (AGAIN) {
+                float a, keep;
+                gate_of(Piece<T>::at(gr[r], j), a, keep);
+                h0[j] = fmaf(a, h0[j], keep * Piece<T>::at(xr[r], j));
+            }
+        }
 #pragma unroll
     for (int r = 0; r < R; ++r) {
         float ox[PER], og[PER];
+        const bool there = t - r < len;
 #pragma unroll
         for (int j = 0; j < PER; ++j) {
             float a, keep;
             gate_of(Piece<T>::at(gr[r], j), a, keep);
             const float l = Piece<T>::at(dr[r], j) + s[j];
-            const float before = t - r > 0 ? Piece<T>::at(hr[r], j) : h0[j];
-            ox[j] = keep * l;
-            og[j] = a * keep * (before - Piece<T>::at(xr[r], j)) * l;
-            s[j] = a * l;
+            ox[j] = there ? keep * l : 0.f;
+            og[j] = there ? a * keep * (hb[r][j] - Piece<T>::at(xr[r], j)) * l : 0.f;
+            if (there) s[j] = a * l;
         }
-        if (t - r >= 0 && left > 0) {
+        if (t - r < p.T && left > 0) {
             Piece<T>::store(dx + (int64_t)(t - r) * p.C, ox, left);
             Piece<T>::store(dg + (int64_t)(t - r) * p.C, og, left);
         }
     }
 }
 
-struct ClearP { u32x4* at; int64_t n; };
-__global__ __launch_bounds__(256) void recur_clear(const ClearP p) {       // ones; the first piece (the ticket) zero
+struct ClearP { u32x4* at; int64_t n, chain; };
+__global__ __launch_bounds__(256) void recur_clear(const ClearP p) {       // ones; the first piece of each chain's space (its ticket) zero
     const int64_t i = (int64_t)blockIdx.x * 256 + threadIdx.x;
-    if (i < p.n) p.at[i] = i ? u32x4{~0u, ~0u, ~0u, ~0u} : u32x4{0, 0, 0, 0};
+    if (i < p.n) p.at[i] = i && i != p.chain ? u32x4{~0u, ~0u, ~0u, ~0u} : u32x4{0, 0, 0, 0};
 }
 
 // ---- host side ---------------------------------------------------------------------------------------------------------------------------
@@ -347,26 +431,43 @@ static Plan plan(const oph_seq_recur* a) {
     l.words = l.blocks > 1 ? l.chains * l.blocks * ch : 0;
     return l;
 }
-static int64_t workspace(const oph_seq_recur* a) {
+// one chain's space: ticket, maps, states
+static int64_t chain_bytes(const Plan& l) { return l.words ? 16 + l.words * 12 : 0; }
+// the gradient in 16 bits: a chain's space for each of its passes, and the states before the stretches
+static int64_t workspace(const oph_seq_recur* a, bool gradient) {
     const Plan l = plan(a);
-    return l.words ? 16 + l.words * 12 : 0;
+    return gradient && type_bytes(a->dtype) == 2 ? 2 * chain_bytes(l) + l.words * (MANY * 8) * (int64_t)sizeof(float) : chain_bytes(l);
 }
-static int start(const oph_seq_recur* a, RecurP& p, void* stream) {          // clears what the blocks hand on
+static void use_chain(RecurP& p, const Plan& l, char* at) {
+    p.ticket = (unsigned*)at;
+    p.map = (unsigned long long*)(at + 16);
+    p.state = (unsigned*)(p.map + l.words);
+}
+static int start(const oph_seq_recur* a, RecurP& p, bool gradient, void* stream) {          // clears what the blocks hand on
     const Plan l = plan(a);
     p.blocks = (int)l.blocks;
     if (!l.words) return OPH_OK;
-    p.ticket = (unsigned*)a->workspace;
-    p.map = (unsigned long long*)((char*)a->workspace + 16);
-    p.state = (unsigned*)(p.map + l.words);
-    const ClearP c = {(u32x4*)a->workspace, workspace(a) / 16};
+    use_chain(p, l, (char*)a->workspace);
+    const int64_t each = chain_bytes(l) / 16;
+    const ClearP c = {(u32x4*)a->workspace, gradient && type_bytes(a->dtype) == 2 ? 2 * each : each, each};
     return launch<ClearP>(recur_clear, dim3((unsigned)cdiv(c.n, 256)), 256, c, 0, stream);
 }
 template <class F> static int run(F one, F many, const oph_seq_recur* a, const RecurP& p, void* stream) {
     const Plan l = plan(a);
     return launch<RecurP>(l.blocks == 1 ? one : many, dim3((unsigned)(l.chains * l.blocks)), 64 * (l.blocks == 1 ? ONE : MANY), p, 0, stream);
 }
-static int check_workspace(const oph_seq_recur* a) {
-    const int64_t need = workspace(a);
+template <class T> static int gradient(const oph_seq_recur* a, RecurP& p, void* stream) {
+    const Plan l = plan(a);
+    if constexpr (sizeof(T) == 2)
+        if (l.words) {
+            p.stretch = (float*)((char*)a->workspace + 2 * chain_bytes(l));
+            if (int rc = launch<RecurP>(recur_forward<T, MANY, true>, dim3((unsigned)(l.chains * l.blocks)), 64 * MANY, p, 0, stream)) return rc;
+            use_chain(p, l, (char*)a->workspace + chain_bytes(l));
+        }
+    return run(recur_gradient<T, ONE>, recur_gradient<T, MANY>, a, p, stream);
+}
+static int check_workspace(const oph_seq_recur* a, bool gradient) {
+    const int64_t need = workspace(a, gradient);
     if (need && (!a->workspace || (int64_t)a->workspace_bytes < need || ((uintptr_t)a->workspace & 15)))
         return fail(OPH_ERR_INVALID, "recurrence: the workspace must hold %lld bytes, 16-byte aligned", (long long)need);
     return OPH_OK;
@@ -378,25 +479,24 @@ using namespace ophseq;
 extern "C" {
 
 int64_t oph_seq_recur_workspace(const oph_seq_recur* a, int gradient) {
-    (void)gradient;                                                       // the same for both
     if (int rc = check(a)) return rc;
-    return workspace(a);
+    return workspace(a, gradient != 0);
 }
 
 int oph_seq_recur_forward(const oph_seq_recur* a, int device, void* stream) {
     if (int rc = check(a)) return rc;
     if (!a->B) return OPH_OK;
     if (!a->h_last || (a->T && (!a->x || !a->gate || !a->h))) return fail(OPH_ERR_INVALID, "recurrence: x, gate, h and h_last must not be NULL");
-    if (int rc = check_workspace(a)) return rc;
+    if (int rc = check_workspace(a, false)) return rc;
     OnDevice on(device);
     if (on.status) return on.status;
     RecurP p = params(a);
     p.h = a->h;
     p.h_last = a->h_last;
-    if (int rc = start(a, p, stream)) return rc;
-    if (a->dtype == OPH_SEQ_F32) return run(recur_forward<float, ONE>, recur_forward<float, MANY>, a, p, stream);
-    if (a->dtype == OPH_SEQ_BF16) return run(recur_forward<bf16_t, ONE>, recur_forward<bf16_t, MANY>, a, p, stream);
-    return run(recur_forward<f16_t, ONE>, recur_forward<f16_t, MANY>, a, p, stream);
+    if (int rc = start(a, p, false, stream)) return rc;
+    if (a->dtype == OPH_SEQ_F32) return run(recur_forward<float, ONE, false>, recur_forward<float, MANY, false>, a, p, stream);
+    if (a->dtype == OPH_SEQ_BF16) return run(recur_forward<bf16_t, ONE, false>, recur_forward<bf16_t, MANY, false>, a, p, stream);
+    return run(recur_forward<f16_t, ONE, false>, recur_forward<f16_t, MANY, false>, a, p, stream);
 }
 
 int oph_seq_recur_gradient(const oph_seq_recur* a, int device, void* stream) {
@@ -404,15 +504,15 @@ int oph_seq_recur_gradient(const oph_seq_recur* a, int device, void* stream) {
     if (!a->B) return OPH_OK;
     if (a->T && (!a->x || !a->gate || !a->h || !a->dh || !a->dx || !a->dgate))
         return fail(OPH_ERR_INVALID, "recurrence: x, gate, h, dh, dx and dgate must not be NULL");
-    if (int rc = check_workspace(a)) return rc;
+    if (int rc = check_workspace(a, true)) return rc;
     OnDevice on(device);
     if (on.status) return on.status;
     RecurP p = params(a);
     p.hin = a->h; p.dh = a->dh; p.dh_last = a->dh_last; p.dx = a->dx; p.dgate = a->dgate; p.dh0 = a->dh0;
-    if (int rc = start(a, p, stream)) return rc;
-    if (a->dtype == OPH_SEQ_F32) return run(recur_gradient<float, ONE>, recur_gradient<float, MANY>, a, p, stream);
-    if (a->dtype == OPH_SEQ_BF16) return run(recur_gradient<bf16_t, ONE>, recur_gradient<bf16_t, MANY>, a, p, stream);
-    return run(recur_gradient<f16_t, ONE>, recur_gradient<f16_t, MANY>, a, p, stream);
+    if (int rc = start(a, p, true, stream)) return rc;
+    if (a->dtype == OPH_SEQ_F32) return gradient<float>(a, p, stream);
+    if (a->dtype == OPH_SEQ_BF16) return gradient<bf16_t>(a, p, stream);
+    return gradient<f16_t>(a, p, stream);
 }
 
 }  // extern "C"

@@ -172,7 +172,8 @@ def gated_recurrence(x, gate, h0=None, lengths=None):
 
 def gated_recurrence_gradient(dh, x, gate, h, h0=None, dh_last=None, lengths=None):
     """Gradient of gated_recurrence: dh (B, T, C) and dh_last (B, C) float32 or None are the gradients of its two results, h its first
-    result.  Returns dx, dgate (B, T, C), 0 past a sequence's length, and dh0 (B, C) float32 (dh_last for a sequence of length 0)."""
+    result (float32: the states that the gradient needs; in 16 bits it forms them again, unrounded, from x, gate and h0).  Returns dx,
+    dgate (B, T, C), 0 past a sequence's length, and dh0 (B, C) float32 (dh_last for a sequence of length 0)."""
     torch = _torch or _setup()
     dtype, device, shape, x, gate, h0, lens = _recur(torch, x, gate, h0, lengths)
     dh, h = _like(torch, "dh", dh, dtype, device, shape), _like(torch, "h", h, dtype, device, shape)

@@ -161,7 +161,7 @@ def recurrence_gradient(dh, dh_last, ctx):
         l, lm = m + d[:, t], big + d[:, t].abs()
         lb = SLACK * per * (2 * cnt + 16 * lm)
         diff = h[:, t] - X[:, t]
-        hb = u * h[:, t].abs() + ctx["state_bound"][:, t] + tiny
+        hb = ctx["state_bound"][:, t] + tiny                        # the float32 state, whatever the forward's result was rounded to
         dx[:, t] = torch.where(on, keep[:, t] * l, z)
         dg[:, t] = torch.where(on, a[:, t] * keep[:, t] * diff * l, z)
         bx[:, t] = torch.where(on, keep[:, t] * lb + u * dx[:, t].abs() + per * dx[:, t].abs(), z) + tiny

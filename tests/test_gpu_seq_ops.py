@@ -577,3 +577,25 @@ def test_attention_padded_rows_of_split_masked_keys(D, dt):
         _within("lse", l, lse, bl)
         for n, g, r, b in zip(("dq", "dk", "dv"), M.cross_attention_gradient(dd, qd, kd, vd, o, l, q_lens=qld, k_lens=kld, key_mask=m), ref, bound):
             _within(n, g, r, b)
+
+
+@dtypes
+@pytest.mark.parametrize("B,T,C", [(2, 200, 40), (2, 700, 72), (1, 3000, 24)], ids=str)
+def test_recurrence_gradient_where_the_state_follows_its_input(B, T, C, dt):
+    """An input that stays for a while and then moves by a step of its type: h_{t-1} - x is far smaller than h, down to less than the half step
+    that h is rounded by in 16 bits, and still has to be that of the float32 state."""
+    from ophelia_amd import modules as M
+    step = torch.finfo(dt).eps
+    gen = torch.Generator().manual_seed(T)
+    moves = torch.randint(0, 3, (B, T, C), generator=gen).float() * (torch.rand(B, T, C, generator=gen) < 0.05)
+    x = (1 + (moves.cumsum(1) % 64) * step).to(dt)
+    g, dh, h0, dl = _rand(2, (B, T, C), dt), _rand(3, (B, T, C), dt), _rand(4, (B, C), torch.float32), _rand(5, (B, C), torch.float32)
+    lens = torch.tensor([T] + [T - 61] * (B - 1), dtype=torch.int32)
+    ref, bound, ctx = O.recurrence(x, g, h0, lens)
+    gref, gbound = O.recurrence_gradient(dh, dl, ctx)
+    xd, gd, dd, h0d, dld, ld = _cuda(x, g, dh, h0, dl, lens)
+    h, last = M.gated_recurrence(xd, gd, h0=h0d, lengths=ld)
+    _within("h", h, ref[0], bound[0])
+    got = M.gated_recurrence_gradient(dd, xd, gd, h, h0=h0d, dh_last=dld, lengths=ld)
+    for n, a, r, b in zip(("dx", "dgate", "dh0"), got, gref, gbound):
+        _within(n, a, r, b)
