@@ -17,6 +17,46 @@ __device__ __forceinline__ float dot8(f32x8 a, f32x8 b) {
     return s;
 }
 
+// Score gradients dS = P (dP - delta) are rounded to the operand type of the next product.  float16 ends at 65504, which they can pass where the
+// gradients that they are summed to do not: every column of a result has a power of two `by` that its dS are multiplied by and that is taken out
+// at the end, both exactly; 1 unless they can pass 2^15.
+// dq, whose column is a query: `by` is lowered when a dS asks for it, and what has been summed is brought to the new one (the running maximum of a
+// softmax, in steps of 2).
+template <class T, int N> __device__ __forceinline__ void into_range(f32x16& S, float& by, f32x16 (&acc)[N]) {
+    if constexpr (__is_same(T, f16_t)) {
+        float top = 0.f;
+#pragma unroll
+        for (int i = 0; i < 16; ++i) top = fmaxf(top, fabsf(S[i]));
+        if (__any(top * by > 32768.f)) {
+            top = fmaxf(top, other_half(top));                              // both halves hold elements of the column
+            const float now = top * by > 32768.f && top < INFINITY ? ldexpf(1.f, 14 - ilogbf(top)) : by;      // what is infinite stays so
+            const float f = now / by;
+#pragma unroll
+            for (int d = 0; d < N; ++d) acc[d] *= f;
+            by = now;
+        }
+        if (__any(by != 1.f)) S *= by;
+    }
+}
+// dk, whose column is a key (its D > 128 form has no register left for that): |dS| <= |dout of the row| |v of the key| + |delta|, since P <= 1.  attn_dq
+// leaves the largest |dout| and |delta| of every 32 rows behind delta, and the bound is known before the first product.  It may be
+// far above the largest dS; what that costs lies below 2^-25 of the bound's 2^15, a 2^-40th of it.  Together (2 x 16 heads over 4 key heads of
+// 4096 x 4096 fp16): x 128 1000 -> 1060 us, x 256 unchanged; dk lowered as dq is spilled 265 registers at x 256, 4010 -> 7600.
+template <class T> __device__ __forceinline__ float* range_of(const AttnP& p, const Where& w, int tiles) {
+    return p.aux + ((int64_t)p.B * p.Hk * p.G * p.Tq + 3) / 4 * 4 + (int64_t)(w.b * p.Hk + w.hk) * tiles * 8;
+}
+template <class T, int N> __device__ __forceinline__ float norm_of(const frag_t<T> (&x)[N]) {
+    float s = 0.f;
+#pragma unroll
+    for (int i = 0; i < N; ++i) s += dot8(__builtin_convertvector(x[i], f32x8), __builtin_convertvector(x[i], f32x8));
+    return sqrtf(s + other_half(s));
+}
+__device__ __forceinline__ float wave_max(float x) {
+#pragma unroll
+    for (int i = 1; i < 64; i <<= 1) x = fmaxf(x, __shfl_xor(x, i));
+    return x;
+}
+
 // ---- dq: S^T = K q^T and dP^T = V dout^T have the queries as columns; dS^T is the operand of dq^T = K^T dS^T -------------------------------
 // 16 bits: waves a SIMD that the registers must leave room for, and rows of a tile in LDS -- D = 64 has few products between two barriers
 // (2 x 16 heads of 4096 x 4096 x 64: 499 us, with tiles of 32 rows 608).
@@ -87,9 +127,16 @@ __global__ __launch_bounds__(256, (grad_waves<T, DP>(3))) void attn_dq(const Att
             if (lse != -INFINITY) lse2 = lse * LOG2E;
         }
         if (r < M && half == 0 && split == 0) p.aux[at] = delta;
+        if constexpr (__is_same(T, f16_t))
+            if (split == 0) {
+                const float n = wave_max(norm_of<T>(dO)), d = wave_max(fabsf(delta));
+                float* to = range_of<T>(p, w, tiles) + (w.tile * 4 + wave) * 2;
+                if (lane == 0) { to[0] = n; to[1] = d; }
+            }
     }
 #pragma unroll
     for (int d = 0; d < DP / 32; ++d) dQ[d] = f32x16{};
+    float by = 1.f;
 
     if (nt) commit(0);
     for (int j = 0; j < nt; ++j) {
@@ -113,6 +160,7 @@ __global__ __launch_bounds__(256, (grad_waves<T, DP>(3))) void attn_dq(const Att
 #pragma unroll
                     for (int i = 0; i < 16; ++i) S[i] = (b >> (8 * (i / 4) + i % 4)) & 1 ? S[i] : 0.f;
                 }
+                into_range<T>(S, by, dQ);
 #pragma unroll
                 for (int s = 0; s < 2; ++s) {
                     const frag_t<T> dS = next_frag<T>(S, s);
@@ -128,13 +176,14 @@ __global__ __launch_bounds__(256, (grad_waves<T, DP>(3))) void attn_dq(const Att
         const int64_t at = (((int64_t)w.b * p.Tq + t) * Hq + h) * p.D;
         T* o = (T*)p.o0 + at;
         float* part = p.part + (int64_t)split * p.B * p.Tq * Hq * p.D + at;
+        const float f = p.scale / by;
 #pragma unroll
         for (int d = 0; d < DP / 32; ++d)
 #pragma unroll
             for (int g = 0; g < 4; ++g) {
                 const int e = 32 * d + 8 * g + 4 * half;
                 f32x4 x = {dQ[d][4 * g], dQ[d][4 * g + 1], dQ[d][4 * g + 2], dQ[d][4 * g + 3]};
-                x = row ? x * p.scale : f32x4{0.f, 0.f, 0.f, 0.f};
+                x = row ? x * f : f32x4{0.f, 0.f, 0.f, 0.f};
                 if (e < p.D) {
                     if (p.nsplit == 1) store4<T>(o + e, x);
                     else *(f32x4*)(part + e) = x;
@@ -219,8 +268,20 @@ __global__ __launch_bounds__(256, (grad_waves<T, DP>(2))) void attn_dkv(const At
     const int64_t kk = min(key, p.Tk - 1);
     row_frags<T, DP>(K, (const T*)p.k + w.b * p.ks[0] + w.hk * p.ks[2] + kk * p.ks[1], p.D, ok, half);
     char* tv = lds + 4 * TB + wave * TV;
+    float by = 1.f;
     if (BOTH || want_dk) {
         row_frags<T, DP>(V, (const T*)p.v + w.b * p.vs[0] + w.hk * p.vs[2] + kk * p.vs[1], p.D, ok, half);
+        if constexpr (__is_same(T, f16_t)) {
+            float n = 0.f, d = 0.f;
+            const int parts = rows ? (p.Tq * p.G + 127) / 128 : 0;
+            const float* from = range_of<T>(p, w, parts);
+            for (int i = lane; i < parts * 4; i += 64) {
+                n = fmaxf(n, from[2 * i]);
+                d = fmaxf(d, from[2 * i + 1]);
+            }
+            const float most = wave_max(n) * norm_of<T>(V) + wave_max(d);
+            if (most > 32768.f && most < INFINITY) by = ldexpf(1.f, 14 - ilogbf(most));
+        }
         if constexpr (VLDS) {
 #pragma unroll
             for (int s = 0; s < DP / 16; ++s) *(frag_t<T>*)(tv + col * Tile<T, DP>::STRIDE + (s * 16 + half * 8) * 2) = V[s];
@@ -264,7 +325,7 @@ __global__ __launch_bounds__(256, (grad_waves<T, DP>(2))) void attn_dkv(const At
                 for (int g = 0; g < 4; ++g) {
                     const f32x4 x = *(const f32x4*)&stat[j & 1][1][q0 + 8 * g + 4 * half];
 #pragma unroll
-                    for (int i = 0; i < 4; ++i) S[4 * g + i] *= dP[4 * g + i] - x[i];
+                    for (int i = 0; i < 4; ++i) S[4 * g + i] *= __is_same(T, f16_t) ? (dP[4 * g + i] - x[i]) * by : dP[4 * g + i] - x[i];
                 }
 #pragma unroll
                 for (int s = 0; s < 2; ++s) {
@@ -285,7 +346,7 @@ __global__ __launch_bounds__(256, (grad_waves<T, DP>(2))) void attn_dkv(const At
             const bool dk = BOTH ? a == 1 : want_dk;
             T* o = (T*)(dk ? p.o1 : p.o0) + at;
             float* part = p.part + ((dk ? p.nsplit : 0) + split) * n + at;
-            const float f = dk ? p.scale : 1.f;
+            const float f = dk ? p.scale / by : 1.f;
 #pragma unroll
             for (int d = 0; d < DP / 32; ++d)
 #pragma unroll
@@ -339,7 +400,11 @@ static GradPlan gradient_plan(const oph_seq_attn* a) {
     g.nk = (int64_t)a->B * a->Tk * a->Hk * a->D;
     return g;
 }
-static int64_t delta_floats(const oph_seq_attn* a) { return cdiv((int64_t)a->B * a->Hq * a->Tq, 4) * 4; }
+// delta, and for float16 the largest |dout| and |delta| of every 32 rows (range_of())
+static int64_t delta_floats(const oph_seq_attn* a) {
+    const int64_t G = a->Hq / a->Hk, range = a->dtype == OPH_SEQ_F16 ? cdiv(a->Tq * G, 128) * 8 * a->B * a->Hk : 0;
+    return cdiv((int64_t)a->B * a->Hq * a->Tq, 4) * 4 + range;
+}
 int64_t attn_gradient_workspace(const oph_seq_attn* a) {
     const GradPlan g = gradient_plan(a);
     const int64_t q = g.dq_split > 1 ? g.dq_split * g.nq : 0, k = g.kv_split > 1 ? 2 * g.kv_split * g.nk : 0;

@@ -88,10 +88,17 @@ def attention_gradient(dout, ctx):
         B, H, T, D_ = x.shape
         return x.reshape(B, H // G, G, T, D_).sum(2)
 
-    bq = SLACK * (u * dq.abs() + dS_bound @ K.abs() + (nk + 20) * E * (dS.abs() @ K.abs())) + f16 * (1 + scale * K.abs().sum(2, keepdim=True))
+    # float16: a score's gradient is held in multiples of 2^-25 as long as all of its row's (dq) lie below 2^15, and what bounds those of its
+    # key (dk); above, the multiples grow with the largest, from 2^14 on
+    wide_q, wide_k = torch.ones(()), torch.ones(())
+    if f16 and nk and nq:
+        wide_q = ((dS / scale).abs().amax(3, keepdim=True) / 2 ** 14).clamp_min(1)
+        most = lambda x: x.reshape(x.shape[0], -1, G).amax(2)[..., None]                  # over a group's heads: (B, Hk, 1)
+        wide_k = ((most(dO.norm(dim=3).amax(2)) * V[:, ::G].norm(dim=3) + most(delta.abs().amax((2, 3)))) / 2 ** 14).clamp_min(1)[..., None]
+    bq = SLACK * (u * dq.abs() + dS_bound @ K.abs() + (nk + 20) * E * (dS.abs() @ K.abs())) + f16 * (1 + wide_q * scale * K.abs().sum(2, keepdim=True))
     bk = SLACK * (u * group(dk).abs() + group(dS_bound.transpose(2, 3) @ Q.abs()) + (nq + 20) * E * group(dS.abs().transpose(2, 3) @ Q.abs()))
     bv = SLACK * (u * group(dv).abs() + group(((relp + n) * P).transpose(2, 3) @ dO.abs()) + (nq + 20) * E * group(P.transpose(2, 3) @ dO.abs()))
-    bk, bv = bk + f16 * (1 + scale * group(Q.abs().sum(2, keepdim=True))), bv + f16 * (1 + group(dO.abs().sum(2, keepdim=True)))
+    bk, bv = bk + f16 * (1 + wide_k * scale * group(Q.abs().sum(2, keepdim=True))), bv + f16 * (1 + group(dO.abs().sum(2, keepdim=True)))
     t = lambda x: x.transpose(1, 2)
     return (t(dq), t(group(dk)), t(group(dv))), (t(bq) + 1e-30, t(bk) + 1e-30, t(bv) + 1e-30)
 

@@ -599,3 +599,26 @@ def test_recurrence_gradient_where_the_state_follows_its_input(B, T, C, dt):
     got = M.gated_recurrence_gradient(dd, xd, gd, h, h0=h0d, dh_last=dld, lengths=ld)
     for n, a, r, b in zip(("dx", "dgate", "dh0"), got, gref, gbound):
         _within(n, a, r, b)
+
+
+@dtypes
+@pytest.mark.parametrize("grows", [False, True], ids=["even", "growing"])
+@pytest.mark.parametrize("shape", [(2, 70, 90, 2, 1, 64), (2, 200, 300, 4, 2, 128), (1, 150, 260, 2, 1, 192), (2, 5, 60, 1, 1, 32), (1, 700, 20, 2, 2, 40)], ids=str)
+def test_attention_gradient_with_large_score_gradients(shape, grows, dt):
+    """Score gradients beyond the range of float16 (65504) whose sums are inside it, all along and from one key and one row to the next."""
+    from ophelia_amd import modules as M
+    B, Tq, Tk, Hq, Hk, D = shape
+    q, k, v, do = (t.float() for t in _case(shape, torch.float32, 17))
+    q, k, v, do = q * 0.01, k * 0.01, v * 100, do * 7000
+    if grows:
+        v, do = v * torch.logspace(-3, 0, Tk)[None, :, None, None], do * torch.logspace(-3, 0, Tq)[None, :, None, None]
+    q, k, v, do = (t.to(dt) for t in (q, k, v, do))
+    ctx = O.attention(q, k, v)[4]
+    ref, bound = O.attention_gradient(do, ctx)
+    top = (ctx["P"] * (do.double().transpose(1, 2) @ ctx["V"].transpose(2, 3))).abs().max()
+    assert top > 2 ** 16 and max(r.abs().max() for r in ref) < 60000, (top, [r.abs().max() for r in ref])
+    qd, kd, vd, dd = _cuda(q, k, v, do)
+    o, l = M.cross_attention(qd, kd, vd)
+    got = M.cross_attention_gradient(dd, qd, kd, vd, o, l)
+    for n, g, r, b in zip(("dq", "dk", "dv"), got, ref, bound):
+        _within(n, g, r, b)
