@@ -9,8 +9,10 @@ Arguments are torch tensors on one GPU: float32, bfloat16 or float16, time-major
 copied together if it is strided itself).  Calls queue kernels on torch's current stream of that GPU and return new tensors; they never
 synchronise, so they can be captured into a graph.  Sums, statistics and states are float32, and no result depends on the order in
 which workgroups run.  Gradients are functions of their own: nothing here records for torch's autograd, and tensors that
-require gradients are refused outside torch.no_grad().  Bad arguments raise ValueError before anything is queued; there is
-no CPU fallback."""
+require gradients are refused outside torch.no_grad().  Bad arguments raise before anything is queued: types, shapes, devices and
+sizes beyond 32 bits ValueError, what the library refuses (head sizes and counts, scales, sizes that it does not do) OpheliaHipError.
+There is no CPU fallback."""
+import ctypes
 import operator
 import struct
 
@@ -75,6 +77,13 @@ def _lens(torch, name, t, device, B):
     return t.contiguous()
 
 
+def _sizes(what, sizes):
+    """The library takes sizes as 32-bit numbers; larger ones (of expanded tensors) must not arrive there as others."""
+    if max(sizes) > 2147483647:
+        raise ValueError("%s: a size of %d, the largest is 2147483647" % (what, max(sizes)))
+    return tuple(sizes)
+
+
 def _ptr(t):
     return 0 if t is None else t.data_ptr()
 
@@ -100,7 +109,7 @@ def embed_lookup(ids, table, scale=1.0, zero_pad=True):
         raise ValueError("table must be (vocab, units), has shape %s" % (tuple(table.shape),))
     table = _like(torch, "table", table, dtype, device, table.shape)
     ids, width = _ids(torch, ids, device)
-    V, U = table.shape
+    V, U = _sizes("table", table.shape)
     out = table.new_empty(ids.shape + (U,))
     _chk(_seq.oph_seq_embed_lookup(ids.data_ptr(), width, ids.numel(), table.data_ptr(), table.stride(0), V, U, float(scale),
                                    bool(zero_pad), _T[dtype], out.data_ptr(), device.index, _stream(device.index)))
@@ -112,17 +121,17 @@ def embed_gradient(ids, dout, vocab, scale=1.0, zero_pad=True):
     scale * the sum of the dout rows whose id is v, taken in float32 in a fixed order.  Rows that no id names, and with zero_pad row 0, are
     zeros; ids outside the table are left out."""
     torch = _torch or _setup()
+    vocab = operator.index(vocab)
+    if vocab < 1 or vocab > 2147483647:
+        raise ValueError("vocab must be a number of rows from 1 to 2147483647, is %d" % vocab)
     dtype, device = _first(torch, "dout", dout)
     ids, width = _ids(torch, ids, device)
     if dout.dim() < 1 or dout.shape[-1] < 1:
         raise ValueError("dout must have a last axis of units, has shape %s" % (tuple(dout.shape),))
-    U = dout.shape[-1]
+    U = _sizes("dout", dout.shape[-1:])[0]
     dout = _like(torch, "dout", dout, dtype, device, ids.shape + (U,))
     if dout.dim() != 2:
         dout = dout.reshape(-1, U)
-    vocab = operator.index(vocab)
-    if vocab < 1:
-        raise ValueError("vocab must be a positive number of rows, is %d" % vocab)
     n = ids.numel()
     nbytes = _chk(_seq.oph_seq_embed_workspace(n, vocab, U))
     ws = _workspace(torch, nbytes, device) if nbytes else None
@@ -138,6 +147,7 @@ def _recur(torch, x, gate, h0, lengths):
     if x.dim() != 3 or x.shape[2] < 1:
         raise ValueError("x must be (batch, time, channels), has shape %s" % (tuple(x.shape),))
     shape = x.shape
+    _sizes("x", shape)
     x = _like(torch, "x", x, dtype, device, shape)
     gate = _like(torch, "gate", gate, dtype, device, shape)
     if h0 is not None:
@@ -197,6 +207,7 @@ def _attention(torch, q, k, v, q_lens, k_lens, key_mask, scale):
         raise ValueError("k must be (batch, time, heads, head size)")
     B, Tq, Hq, D = q.shape
     Tk, Hk = k.shape[1], k.shape[2]
+    _sizes("q and k", (B, Tq, Tk, Hq, Hk, D))
     shape = (B, Tk, Hk, D)
     q = _like(torch, "q", q, dtype, device, q.shape)
     k, v = _like(torch, "k", k, dtype, device, shape), _like(torch, "v", v, dtype, device, shape)
@@ -204,7 +215,8 @@ def _attention(torch, q, k, v, q_lens, k_lens, key_mask, scale):
     if key_mask is not None and (not isinstance(key_mask, torch.Tensor) or key_mask.dtype not in (torch.bool, torch.uint8) or
                                  key_mask.device != device or key_mask.shape != (B, Tk)):
         raise ValueError("key_mask must be a bool tensor of shape (%d, %d) on %s" % (B, Tk, device))
-    sizes = (B, Tq, Tk, Hq, Hk, D, _T[dtype], D ** -0.5 if scale is None and D else float(scale or 0.0))
+    # a scale that float32 does not hold is infinite there, which the library refuses
+    sizes = (B, Tq, Tk, Hq, Hk, D, _T[dtype], D ** -0.5 if scale is None and D else ctypes.c_float(scale or 0.0).value)
     return dtype, device, q, k, v, ql, kl, sizes
 
 

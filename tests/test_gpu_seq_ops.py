@@ -622,3 +622,22 @@ def test_attention_gradient_with_large_score_gradients(shape, grows, dt):
     got = M.cross_attention_gradient(dd, qd, kd, vd, o, l)
     for n, g, r, b in zip(("dq", "dk", "dv"), got, ref, bound):
         _within(n, g, r, b)
+
+
+def test_refusals_of_sizes_and_scales_beyond_32_bits():
+    """Expanded tensors can have any size without memory: what does not fit the library's numbers is refused as documented."""
+    from ophelia_amd import _lib
+    from ophelia_amd import modules as M
+    ids, one = torch.zeros(2, dtype=torch.int32, device="cuda"), torch.zeros(1, 1, 1, 8, device="cuda")
+    far = 2 ** 32 + 4
+    for call in (lambda: M.embed_lookup(ids, one[0, 0].expand(far, 8)), lambda: M.embed_gradient(ids, one[0, 0].expand(2, 8), far),
+                 lambda: M.cross_attention(one, one.expand(1, far, 1, 8), one.expand(1, far, 1, 8)),
+                 lambda: M.cross_attention(one.expand(far, 1, 1, 8), one.expand(far, 1, 1, 8), one.expand(far, 1, 1, 8)),
+                 lambda: M.cross_attention_gradient(one, one, one.expand(1, far, 1, 8), one.expand(1, far, 1, 8), one, one[:, :, :, 0]),
+                 lambda: M.gated_recurrence(one[0].expand(1, far, 8), one[0].expand(1, far, 8)),
+                 lambda: M.gated_recurrence_gradient(*[one[0].expand(1, far, 8)] * 4)):
+        with pytest.raises(ValueError):
+            call()
+    for scale in (1e300, -1e300, 1e-60, math.inf, math.nan, 0.0):
+        with pytest.raises(_lib.OpheliaHipError):
+            M.cross_attention(one, one, one, scale=scale)

@@ -177,3 +177,16 @@ int main() {
                     str(src), "-o", exe], check=True, timeout=120)
     r = subprocess.run([exe], capture_output=True, text=True, timeout=120)
     assert r.returncode == 0, (r.stdout[-500:], r.stderr[-1500:])
+
+
+def test_sizes_beyond_32_bits_are_refused():
+    """The C ABI takes sizes as 32-bit numbers: 2^32 + 4 rows must not arrive as 4."""
+    from ophelia_amd import device_ops
+    from ophelia_amd import modules as M
+    ids, dout = torch.zeros(2, dtype=torch.int32), torch.zeros(2, 4)
+    for vocab in (2 ** 32 + 4, 2 ** 31, 0, -1):
+        with pytest.raises(ValueError, match="vocab"):
+            M.embed_gradient(ids, dout, vocab)
+    assert device_ops._sizes("x", (3, 2 ** 31 - 1)) == (3, 2 ** 31 - 1)
+    with pytest.raises(ValueError, match="2147483648"):
+        device_ops._sizes("x", (3, 2 ** 31))
