@@ -8,8 +8,8 @@ without leaving the GPU.  ophelia_amd.modules offers them beside the host-buffer
 Arguments are torch tensors on one GPU: float32, bfloat16 or float16, time-major views and other strides welcome (the last axis is
 copied together if it is strided itself).  Calls queue kernels on torch's current stream of that GPU and return new tensors; they never
 synchronise, so they can be captured into a graph.  Sums, statistics and states are float32, and no result depends on the order in
-which workgroups run.  Gradients are functions of their own: nothing here records for torch's autograd, and tensors that
-require gradients are refused outside torch.no_grad().  Bad arguments raise before anything is queued: types, shapes, devices and
+which workgroups run.  Gradients are functions of their own: nothing here records for torch's autograd, tensors that require
+gradients are refused outside torch.no_grad(), and tensors that carry a forward-mode tangent always.  Bad arguments raise before anything is queued: types, shapes, devices and
 sizes beyond 32 bits ValueError, what the library refuses (head sizes and counts, scales, sizes that it does not do) OpheliaHipError.
 There is no CPU fallback."""
 import ctypes
@@ -22,6 +22,7 @@ _T = {}
 _torch = None                 # the module, and below the library and the stream's raw handle: found at the first call
 _seq = None
 _stream = None
+_forward = None               # torch.autograd.forward_ad
 # the argument structures of include/ophelia_seq.h as the compiler lays them out: packing them in one go is a third of the time that filling
 # ctypes fields takes, and a call on small tensors is bound by what happens here
 _ATTN = struct.Struct("@12P14qPN7if")
@@ -29,8 +30,9 @@ _RECUR = struct.Struct("@11P8qPN4i")
 
 
 def _setup():
-    global _torch, _seq, _stream
+    global _torch, _seq, _stream, _forward
     import torch
+    _forward = torch.autograd.forward_ad
     _T.update({torch.float32: _lib.SEQ_F32, torch.bfloat16: _lib.SEQ_BF16, torch.float16: _lib.SEQ_F16})
     # the raw handle of the current stream without the stream object around it, where this torch has it
     _stream = getattr(torch._C, "_cuda_getCurrentRawStream", None) or (lambda index: torch.cuda.current_stream(index).cuda_stream)
@@ -56,7 +58,7 @@ def _first(torch, name, t):
 
 def _like(torch, name, t, dtype, device, shape):
     """A tensor of the call: type, device and shape as given, unit stride in the last axis."""
-    if isinstance(t, torch.Tensor) and t.dtype is dtype and t.shape == shape and t.device == device and not t.requires_grad:
+    if isinstance(t, torch.Tensor) and t.dtype is dtype and t.shape == shape and t.device == device and not t.requires_grad and _forward._current_level < 0:
         return t if t.stride(-1) == 1 or t.shape[-1] == 1 else t.contiguous()
     if not isinstance(t, torch.Tensor) or t.dtype != dtype:
         raise ValueError("%s must be a %s tensor" % (name, dtype))
@@ -64,8 +66,10 @@ def _like(torch, name, t, dtype, device, shape):
         raise ValueError("%s is on %s, the call on %s" % (name, t.device, device))
     if t.shape != shape:
         raise ValueError("%s has shape %s, expected %s" % (name, tuple(t.shape), tuple(shape)))
-    if torch.is_grad_enabled():
+    if t.requires_grad and torch.is_grad_enabled():
         raise ValueError("%s requires a gradient: call under torch.no_grad() and use the gradient function" % name)
+    if _forward._current_level >= 0 and _forward.unpack_dual(t).tangent is not None:      # not a matter of no_grad()
+        raise ValueError("%s carries a forward-mode tangent, which would be lost: unpack it first" % name)
     return t if t.stride(-1) == 1 or t.shape[-1] == 1 else t.contiguous()
 
 

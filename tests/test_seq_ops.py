@@ -190,3 +190,22 @@ def test_sizes_beyond_32_bits_are_refused():
     assert device_ops._sizes("x", (3, 2 ** 31 - 1)) == (3, 2 ** 31 - 1)
     with pytest.raises(ValueError, match="2147483648"):
         device_ops._sizes("x", (3, 2 ** 31))
+
+
+def test_forward_mode_tangents_are_refused():
+    """A dual tensor does not require a gradient: its tangent must not get lost in silence, under no_grad() neither."""
+    from ophelia_amd import device_ops
+    device_ops._torch or device_ops._setup()
+    ad = torch.autograd.forward_ad
+    look = lambda t: device_ops._like(torch, "q", t, torch.float32, t.device, t.shape)
+    with ad.dual_level():
+        plain, dual = torch.ones(2, 3), ad.make_dual(torch.ones(2, 3), torch.ones(2, 3))
+        assert look(plain) is plain and look(ad.unpack_dual(dual).primal).shape == (2, 3)
+        with pytest.raises(ValueError, match="tangent"):
+            look(dual)
+        with torch.no_grad(), pytest.raises(ValueError, match="tangent"):
+            look(dual)
+    with pytest.raises(ValueError, match="gradient"):
+        look(torch.ones(2, requires_grad=True))
+    with torch.no_grad():
+        assert look(torch.ones(2, requires_grad=True)).shape == (2,)
