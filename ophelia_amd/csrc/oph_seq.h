@@ -78,6 +78,7 @@ __device__ __forceinline__ float other_half(float x) { return __shfl_xor(x, 32);
 
 // ---- host side ---------------------------------------------------------------------------------------------------------------
 int fail(int status, const char* fmt, ...) __attribute__((format(printf, 2, 3)));
+int device_fail(hipError_t e, const char* what);
 int type_bytes(int dtype);        // 0: not a type
 
 // makes `device` current for the life of the object
@@ -91,7 +92,7 @@ template <class P> int launch(void (*kernel)(P), dim3 grid, int threads, const P
     P arg = p;
     void* args[] = {&arg};
     const hipError_t e = hipLaunchKernel((const void*)kernel, grid, dim3((unsigned)threads), args, lds, (hipStream_t)stream);
-    return e == hipSuccess ? 0 : fail(-3 /* OPH_ERR_DEVICE */, "kernel launch: %s", hipGetErrorString(e));
+    return e == hipSuccess ? 0 : device_fail(e, "kernel launch");
 }
 
 inline int64_t cdiv(int64_t a, int64_t b) { return (a + b - 1) / b; }

@@ -19,11 +19,18 @@ int fail(int status, const char* fmt, ...) {
 
 int type_bytes(int dtype) { return dtype == OPH_SEQ_F32 ? 4 : dtype == OPH_SEQ_BF16 || dtype == OPH_SEQ_F16 ? 2 : 0; }
 
+// An error of the runtime goes to the caller as this call's, and is taken from the runtime: its next reader would report it as its own.
+int device_fail(hipError_t e, const char* what) {
+    (void)hipGetLastError();
+    return fail(OPH_ERR_DEVICE, "%s: %s", what, hipGetErrorString(e));
+}
+
 OnDevice::OnDevice(int device) {
     int now = -1;
-    if (hipGetDevice(&now) != hipSuccess) { status = fail(OPH_ERR_DEVICE, "no usable HIP device (no CPU fallback)"); return; }
+    if (hipError_t e = hipGetDevice(&now)) { status = device_fail(e, "no usable HIP device (no CPU fallback)"); return; }
     if (now == device) return;
-    if (device < 0 || hipSetDevice(device) != hipSuccess) { status = fail(OPH_ERR_DEVICE, "device %d cannot be used", device); return; }
+    if (device < 0) { status = fail(OPH_ERR_DEVICE, "device %d cannot be used", device); return; }
+    if (hipError_t e = hipSetDevice(device)) { status = device_fail(e, "the device cannot be used"); return; }
     before = now;
 }
 OnDevice::~OnDevice() {

@@ -641,3 +641,17 @@ def test_refusals_of_sizes_and_scales_beyond_32_bits():
     for scale in (1e300, -1e300, 1e-60, math.inf, math.nan, 0.0):
         with pytest.raises(_lib.OpheliaHipError):
             M.cross_attention(one, one, one, scale=scale)
+
+
+def test_a_refused_device_leaves_no_error_behind():
+    """What the runtime answers to a device that is not there is reported by the call, and not once more by the caller's next GPU call."""
+    from ophelia_amd import _lib
+    lib = _lib.load_seq()
+    ids, table = torch.ones(2, dtype=torch.int32, device="cuda"), torch.ones(3, 4, device="cuda")
+    out = torch.zeros(2, 4, device="cuda")
+    torch.cuda.synchronize()
+    for device in (1000, -1):
+        rc = lib.oph_seq_embed_lookup(ids.data_ptr(), 4, 2, table.data_ptr(), 4, 3, 4, 1.0, 1, 0, out.data_ptr(), device, None)
+        assert rc == -3 and "device" in lib.oph_seq_last_error().decode()
+        assert (table + 1).sum().item() == 24                              # torch asks for the last error after every launch
+        assert not out.any()
