@@ -4,6 +4,8 @@
 
 #include <math.h>
 
+#include <algorithm>
+
 namespace ophseq {
 
 // Running softmax of one query column: m in units of log2, l the sum over this lane's half of the keys.
@@ -333,7 +335,12 @@ int attn_check(const oph_seq_attn* a, bool gradient) {
     if ((double)a->Tq * a->Hq / a->Hk * (a->Hq / a->Hk) > 2147483647.0 || (double)a->B * a->Hq * ((double)a->Tq + a->Tk + 64) > 4.0e9 || a->Tk > 2147483000 - 256 ||
         a->Tq > 2147483000 - 256 || (double)a->B * a->Hq > 1.0e7)
         return fail(OPH_ERR_UNSUPPORTED, "attention: too many rows (B %d, Tq %d, Tk %d, Hq %d)", a->B, a->Tq, a->Tk, a->Hq);
-    (void)gradient;
+    // a launch has less than 2^32 threads: 256 for 128 rows or keys (fp32, D > 128: 16; 16 bits, D > 128: twice for keys), 512 for the few rows of
+    // a head
+    const int64_t heads = (int64_t)a->B * a->Hk, unit = gradient && a->dtype == OPH_SEQ_F32 && a->D > 128 ? 16 : 128;
+    const int64_t rows = cdiv((int64_t)a->Tq * (a->Hq / a->Hk), unit), keys = gradient ? cdiv(a->Tk, unit) * (a->D > 128 && unit == 128 ? 2 : 1) : 0;
+    if (std::max(std::max(rows, keys) * 256, (int64_t)512) * heads >= 1ll << 32)
+        return fail(OPH_ERR_UNSUPPORTED, "attention: too many rows for one launch (B %d, Tq %d, Tk %d, Hq %d)", a->B, a->Tq, a->Tk, a->Hq);
     return OPH_OK;
 }
 

@@ -209,3 +209,18 @@ def test_forward_mode_tangents_are_refused():
         look(torch.ones(2, requires_grad=True))
     with torch.no_grad():
         assert look(torch.ones(2, requires_grad=True)).shape == (2,)
+
+
+@pytest.mark.parametrize("over", [dict(B=2, Hq=1, Hk=1, D=8, Tq=1200000000, Tk=1), dict(B=9000, Hq=1000, Hk=1000, Tq=1, Tk=1),
+                                  dict(B=2, Hq=1, Hk=1, D=8, Tq=1, Tk=1200000000), dict(B=1, Hq=1, Hk=1, D=136, dtype=0, Tq=300000000, Tk=1),
+                                  dict(B=2, Hq=1, Hk=1, D=136, Tq=1, Tk=600000000)], ids=str)
+def test_attention_refuses_what_one_launch_does_not_hold(lib, over):
+    """A launch has less than 2^32 threads: what needs more is refused before anything is launched, not half way through a gradient.  Long
+    keys do not bound the forward, nor long rows of fp32 heads above 128."""
+    a = _attn(workspace=4096, workspace_bytes=1 << 50, **over)
+    assert lib.oph_seq_attn_gradient(C.byref(a), 0, None) == -4 and "too many" in lib.oph_seq_last_error().decode()
+    assert lib.oph_seq_attn_workspace(C.byref(a), 1) == -4
+    if over["Tq"] == 1 and over["Tk"] > 1 or over.get("dtype") == 0:
+        assert lib.oph_seq_attn_workspace(C.byref(a), 0) >= 0
+    else:
+        assert lib.oph_seq_attn_forward(C.byref(a), 0, None) == -4
