@@ -655,3 +655,59 @@ def test_a_refused_device_leaves_no_error_behind():
         assert rc == -3 and "device" in lib.oph_seq_last_error().decode()
         assert (table + 1).sum().item() == 24                              # torch asks for the last error after every launch
         assert not out.any()
+
+
+# shapes that give a wave of every forward kernel several tiles of keys: shared tiles (with 5 or more, and a remainder), split keys, 16 rows, few rows
+LONG = [(8, 130, 333, 16, 16, 64), (8, 70, 333, 32, 16, 72), (8, 130, 333, 16, 16, 128), (16, 130, 170, 8, 8, 192), (2, 33, 700, 2, 2, 64),
+        (2, 40, 800, 4, 2, 128), (1, 33, 1400, 1, 1, 256), (2, 1, 900, 2, 1, 64), (2, 2, 3000, 4, 2, 128), (3, 300, 450, 1, 1, 40)]
+
+
+@dtypes
+@pytest.mark.parametrize("kind", ["even", "growing", "falling", "masked"])
+@pytest.mark.parametrize("shape", LONG, ids=str)
+def test_attention_where_the_maximum_moves_from_tile_to_tile(shape, kind, dt):
+    """Scores whose maximum rises (or falls) by more than 2^8 from one tile of keys to the next, several times along the keys, or does neither; masked: it rises,
+    with whole tiles and every third key of the others left out, and ragged lengths."""
+    from ophelia_amd import modules as M
+    B, Tq, Tk, Hq, Hk, D = shape
+    q, k, v, do = _case(shape, torch.float32, 23)
+    size = torch.linspace(0.1, 20.0, Tk)[None, :, None, None]
+    k = k if kind == "even" else k * (size.flip(1) if kind == "falling" else size)
+    q, k, v, do = (t.to(dt) for t in (q, k, v, do))
+    ql = kl = mask = None
+    if kind == "masked":
+        g = torch.Generator().manual_seed(3)
+        ql, kl = (torch.randint(n // 2, n + 1, (B,), generator=g, dtype=torch.int32) for n in (Tq, Tk))
+        mask = torch.ones(B, Tk, dtype=torch.bool)
+        mask[:, ::3] = mask[:, :70] = mask[:, 128:192] = False
+    out, lse, bo, bl, ctx = O.attention(q, k, v, ql, kl, mask)
+    ref, bound = O.attention_gradient(do, ctx)
+    qd, kd, vd, dd, qld, kld, md = _cuda(q, k, v, do, ql, kl, mask)
+    o, l = M.cross_attention(qd, kd, vd, q_lens=qld, k_lens=kld, key_mask=md)
+    _within("out", o, out, bo)
+    _within("lse", l, lse, bl)
+    for n, g, r, b in zip(("dq", "dk", "dv"), M.cross_attention_gradient(dd, qd, kd, vd, o, l, q_lens=qld, k_lens=kld, key_mask=md), ref, bound):
+        _within(n, g, r, b)
+
+
+@dtypes
+@pytest.mark.parametrize("T", [1, 40, 600])
+def test_recurrence_state_updated_in_place(T, dt):
+    """The C ABI lets h0 be h_last's buffer: the state of a decoder, one block and several."""
+    import ctypes as C
+    from ophelia_amd import _lib
+    from ophelia_amd import modules as M
+    B, Ch = 3, 50
+    x, g, state = _rand(1, (B, T, Ch), dt).cuda(), _rand(2, (B, T, Ch), dt).cuda(), _rand(3, (B, Ch), torch.float32).cuda()
+    lens = torch.tensor([T, 0, (T + 1) // 2], dtype=torch.int32, device="cuda")
+    h, last = M.gated_recurrence(x, g, h0=state, lengths=lens)
+    lib, a = _lib.load_seq(), _lib.OphSeqRecur()
+    out = torch.empty_like(x)
+    a.x, a.gate, a.h0, a.h, a.h_last, a.lens = x.data_ptr(), g.data_ptr(), state.data_ptr(), out.data_ptr(), state.data_ptr(), lens.data_ptr()
+    a.x_stride[:], a.gate_stride[:] = x.stride()[:2], g.stride()[:2]
+    a.B, a.T, a.C, a.dtype = B, T, Ch, DT.index(dt)
+    need = lib.oph_seq_recur_workspace(C.byref(a), 0)
+    ws = torch.empty(max(need, 16), dtype=torch.uint8, device="cuda")
+    a.workspace, a.workspace_bytes = ws.data_ptr(), need
+    assert lib.oph_seq_recur_forward(C.byref(a), 0, torch.cuda.current_stream().cuda_stream) == 0
+    assert torch.equal(out, h) and torch.equal(state, last)
