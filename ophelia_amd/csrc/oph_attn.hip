@@ -46,18 +46,18 @@ template <int N> __device__ __forceinline__ float soft_step(f32x16 (&S)[N], uint
     return shrink;
 }
 
-// ---- many rows: a workgroup of 4 waves, 32*NQ rows each, over all keys; key and value tiles in LDS for the four -----------------------
+// ---- many rows: a workgroup of 4 waves, 32 rows each, over all keys; key and value tiles in LDS for the four -------------------------
 // waves a SIMD that the registers must leave room for: a second wave's products run under the first one's exponentials (4 x 16 heads
 // of 4096 x 4096 x 128: 576 us with two waves, 970 with one; D = 64: three)
 template <class T, int DP> constexpr int wide_waves() { return sizeof(T) == 4 || DP > 128 ? 1 : DP > 64 ? 2 : 3; }
-template <class T, int DP, int KT, int NQ>
+template <class T, int DP, int KT>
 __global__ __launch_bounds__(256, (wide_waves<T, DP>())) void attn_wide(const AttnP p) {
-    constexpr int ROWS = 128 * NQ, NK = KT / 32, TB = Tile<T, DP>::bytes(KT);
+    constexpr int ROWS = 128, NK = KT / 32, TB = Tile<T, DP>::bytes(KT);
     __shared__ __attribute__((aligned(16))) char lds[4 * TB];
     const int tid = threadIdx.x, lane = tid & 63, wave = tid >> 6, half = lane >> 5, col = lane & 31;
     const int M = p.Tq * p.G, tiles = (M + ROWS - 1) / ROWS;
     const Where w = where(p, on_xcd(p, blockIdx.x, tiles * p.B * p.Hk), tiles);
-    const int row0 = w.tile * ROWS + wave * 32 * NQ;
+    const int r = w.tile * ROWS + wave * 32 + col, t = row_time(p, r), h = w.hk * p.G + r - t * p.G;
     const float c = p.scale * LOG2E;
 
     const T* k = (const T*)p.k + w.b * p.ks[0] + w.hk * p.ks[2];
@@ -78,28 +78,23 @@ __global__ __launch_bounds__(256, (wide_waves<T, DP>())) void attn_wide(const At
             v1 += KT * p.vs[1];
             return;
         }
-        sk.load([&](int r) { return k + (int64_t)min(key0 + r, last) * p.ks[1]; }, p.D, tid);
-        sv.load([&](int r) { return v + (int64_t)min(key0 + r, last) * p.vs[1]; }, p.D, tid);
+        sk.load([&](int i) { return k + (int64_t)min(key0 + i, last) * p.ks[1]; }, p.D, tid);
+        sv.load([&](int i) { return v + (int64_t)min(key0 + i, last) * p.vs[1]; }, p.D, tid);
     };
     auto commit = [&](int j) {
-        char* t = lds + (j & 1) * 2 * TB;
+        char* x = lds + (j & 1) * 2 * TB;
         bits = key_bits(byte, j * KT, w.klen, lane) & (KT == 64 ? ~0ull : 0xffffffffull);
-        sk.store(t, bits, p.D, tid);
-        sv.store(t + TB, bits, p.D, tid);
+        sk.store(x, bits, p.D, tid);
+        sv.store(x + TB, bits, p.D, tid);
     };
     if (nt) fetch(0);                                    // on its way while the rows' operands are loaded
 
-    frag_t<T> Q[NQ][DP / 16];
-    f32x16 O[NQ][DP / 32];
-    Soft st[NQ];
+    frag_t<T> Q[DP / 16];
+    f32x16 O[DP / 32];
+    Soft st = {-INFINITY, 0.f};
+    row_frags<T, DP>(Q, row_ptr<T>(p, p.q, w, r, p.qs[0], p.qs[1], p.qs[2]), p.D, r < M && t < w.qlen, half);
 #pragma unroll
-    for (int n = 0; n < NQ; ++n) {
-        const int r = row0 + n * 32 + col;
-        row_frags<T, DP>(Q[n], row_ptr<T>(p, p.q, w, r, p.qs[0], p.qs[1], p.qs[2]), p.D, r < M && row_time(p, r) < w.qlen, half);
-        st[n] = Soft{-INFINITY, 0.f};
-#pragma unroll
-        for (int d = 0; d < DP / 32; ++d) O[n][d] = f32x16{};
-    }
+    for (int d = 0; d < DP / 32; ++d) O[d] = f32x16{};
 
     if (nt) commit(0);
     for (int j = 0; j < nt; ++j) {
@@ -107,66 +102,45 @@ __global__ __launch_bounds__(256, (wide_waves<T, DP>())) void attn_wide(const At
         __syncthreads();
         if (j + 1 < nt) fetch(j + 1);
         if (now) {
-            const char* tk = lds + (j & 1) * 2 * TB;
-            f32x16 S[NQ][NK];
+            const char *tk = lds + (j & 1) * 2 * TB, *tv = tk + TB;
+            f32x16 S[NK];
 #pragma unroll
-            for (int n = 0; n < NQ; ++n)
-#pragma unroll
-                for (int i = 0; i < NK; ++i) S[n][i] = f32x16{};
+            for (int i = 0; i < NK; ++i) S[i] = f32x16{};
 #pragma unroll
             for (int s = 0; s < DP / 16; ++s)
 #pragma unroll
-                for (int i = 0; i < NK; ++i) {
-                    const frag_t<T> a = row_frag<T, DP>(tk, 32 * i, s, lane);
+                for (int i = 0; i < NK; ++i) S[i] = El<T>::mma(row_frag<T, DP>(tk, 32 * i, s, lane), Q[s], S[i]);
+            const float shrink = soft_step<NK>(S, now, st, c, half);
+            if (__any(shrink != 1.f)) {
 #pragma unroll
-                    for (int n = 0; n < NQ; ++n) S[n][i] = El<T>::mma(a, Q[n][s], S[n][i]);
-                }
-#pragma unroll
-            for (int n = 0; n < NQ; ++n) {
-                const float shrink = soft_step<NK>(S[n], now, st[n], c, half);
-                if (__any(shrink != 1.f)) {
-#pragma unroll
-                    for (int d = 0; d < DP / 32; ++d) O[n][d] *= shrink;
-                }
+                for (int d = 0; d < DP / 32; ++d) O[d] *= shrink;
             }
-            const char* tv = tk + TB;
 #pragma unroll
             for (int i = 0; i < NK; ++i)
 #pragma unroll
                 for (int s = 0; s < 2; ++s) {
-                    frag_t<T> P[NQ];
+                    const frag_t<T> P = next_frag<T>(S[i], s);
 #pragma unroll
-                    for (int n = 0; n < NQ; ++n) P[n] = next_frag<T>(S[n][i], s);
-#pragma unroll
-                    for (int d = 0; d < DP / 32; ++d) {
-                        const frag_t<T> a = trans_frag<T, DP>(tv, 32 * i + 16 * s, 32 * d, lane);
-#pragma unroll
-                        for (int n = 0; n < NQ; ++n) O[n][d] = El<T>::mma(a, P[n], O[n][d]);
-                    }
+                    for (int d = 0; d < DP / 32; ++d) O[d] = El<T>::mma(trans_frag<T, DP>(tv, 32 * i + 16 * s, 32 * d, lane), P, O[d]);
                 }
         }
         if (j + 1 < nt) commit(j + 1);
     }
 
+    const float l = st.l + other_half(st.l);
+    if (r < M) {
+        const bool live = t < w.qlen && l != 0.f;                          // NaN stays NaN
+        const float inv = live ? 1.f / l : 0.f;
+        T* o = (T*)p.o0 + (((int64_t)w.b * p.Tq + t) * (p.Hk * p.G) + h) * p.D;
 #pragma unroll
-    for (int n = 0; n < NQ; ++n) {
-        const int r = row0 + n * 32 + col;
-        const float l = st[n].l + other_half(st[n].l);
-        const int t = row_time(p, r), h = w.hk * p.G + r - t * p.G;
-        if (r < M) {
-            const bool live = t < w.qlen && l != 0.f;                  // NaN stays NaN
-            const float inv = live ? 1.f / l : 0.f;
-            T* o = (T*)p.o0 + (((int64_t)w.b * p.Tq + t) * (p.Hk * p.G) + h) * p.D;
+        for (int d = 0; d < DP / 32; ++d)
 #pragma unroll
-            for (int d = 0; d < DP / 32; ++d)
-#pragma unroll
-                for (int g = 0; g < 4; ++g) {
-                    const int at = 32 * d + 8 * g + 4 * half;
-                    const f32x4 x = {O[n][d][4 * g], O[n][d][4 * g + 1], O[n][d][4 * g + 2], O[n][d][4 * g + 3]};
-                    if (at < p.D) store4<T>(o + at, live ? x * inv : f32x4{0.f, 0.f, 0.f, 0.f});
-                }
-            if (half == 0) p.lse[((int64_t)w.b * (p.Hk * p.G) + h) * p.Tq + t] = live ? (st[n].m + log2f(l)) * LN2 : -INFINITY;
-        }
+            for (int g = 0; g < 4; ++g) {
+                const int at = 32 * d + 8 * g + 4 * half;
+                const f32x4 x = {O[d][4 * g], O[d][4 * g + 1], O[d][4 * g + 2], O[d][4 * g + 3]};
+                if (at < p.D) store4<T>(o + at, live ? x * inv : f32x4{0.f, 0.f, 0.f, 0.f});
+            }
+        if (half == 0) p.lse[((int64_t)w.b * (p.Hk * p.G) + h) * p.Tq + t] = live ? (st.m + log2f(l)) * LN2 : -INFINITY;
     }
 }
 
@@ -392,10 +366,10 @@ int64_t attn_forward_workspace(const oph_seq_attn* a) {
     return f.nsplit == 1 ? 0 : f.units * f.nsplit * f.rows * (pad_d(a->D) + 2) * (int64_t)sizeof(float);
 }
 
-template <class T, int DP, int KT, int NQ> static int forward(const oph_seq_attn* a, const FwdPlan& f, AttnP& p, void* stream) {
-    const int64_t M = (int64_t)p.Tq * p.G, heads = (int64_t)p.B * p.Hk, groups = f.wide ? cdiv(M, 128 * NQ) * heads : f.units * f.nsplit;
+template <class T, int DP, int KT> static int forward(const oph_seq_attn* a, const FwdPlan& f, AttnP& p, void* stream) {
+    const int64_t M = (int64_t)p.Tq * p.G, heads = (int64_t)p.B * p.Hk, groups = f.wide ? cdiv(M, 128) * heads : f.units * f.nsplit;
     p.chunk = run_of(a, groups, f.few);
-    if (f.wide) return launch<AttnP>(attn_wide<T, DP, KT, NQ>, dim3((unsigned)groups), 256, p, 0, stream);
+    if (f.wide) return launch<AttnP>(attn_wide<T, DP, KT>, dim3((unsigned)groups), 256, p, 0, stream);
     p.nsplit = f.nsplit;
     p.part = (float*)a->workspace;
     p.aux = p.part + f.units * f.nsplit * f.rows * DP;
@@ -409,9 +383,9 @@ template <class T, int DP, int KT, int NQ> static int forward(const oph_seq_attn
 }
 template <class T> static int forward_d(const oph_seq_attn* a, const FwdPlan& f, AttnP& p, void* stream) {
     constexpr int KT = sizeof(T) == 2 ? 64 : 32;
-    if (p.D <= 64) return forward<T, 64, 64, 1>(a, f, p, stream);
-    if (p.D <= 128) return forward<T, 128, KT, 1>(a, f, p, stream);
-    return forward<T, 256, 32, 1>(a, f, p, stream);
+    if (p.D <= 64) return forward<T, 64, 64>(a, f, p, stream);
+    if (p.D <= 128) return forward<T, 128, KT>(a, f, p, stream);
+    return forward<T, 256, 32>(a, f, p, stream);
 }
 
 }  // namespace ophseq
