@@ -711,3 +711,39 @@ def test_recurrence_state_updated_in_place(T, dt):
     a.workspace, a.workspace_bytes = ws.data_ptr(), need
     assert lib.oph_seq_recur_forward(C.byref(a), 0, torch.cuda.current_stream().cuda_stream) == 0
     assert torch.equal(out, h) and torch.equal(state, last)
+
+
+@pytest.mark.parametrize("dt", DT[1:], ids=IDS[1:])
+def test_long_16_bit_gradients_in_two_graphs(dt):
+    """The gradients whose launches hand each other states, norms and parts through a workspace, captured twice: every replay has the eager
+    call's bits for the inputs it finds, with eager work on another size in between."""
+    from ophelia_amd import modules as M
+    x, g, dh = (_rand(s, (2, 600, 72), dt).cuda() for s in (1, 2, 3))
+    h0 = _rand(4, (2, 72), torch.float32).cuda()
+    lens = torch.tensor([600, 333], dtype=torch.int32, device="cuda")
+    q, k, v, do = _cuda(*_case((2, 90, 700, 4, 2, 64), dt, 5))
+
+    def go():
+        h, last = M.gated_recurrence(x, g, h0=h0, lengths=lens)
+        o, l = M.cross_attention(q, k, v)
+        return [h, last, *M.gated_recurrence_gradient(dh, x, g, h, h0=h0, lengths=lens), o, l, *M.cross_attention_gradient(do, q, k, v, o, l)]
+
+    go()
+    graphs = []
+    for _ in range(2):
+        gr = torch.cuda.CUDAGraph()
+        with torch.cuda.graph(gr):
+            res = go()
+        graphs.append((gr, res))
+    for i in range(4):
+        x.copy_(_rand(20 + i, x.shape, dt))
+        do.copy_(_rand(30 + i, do.shape, dt, 10.0 ** (i + 1)))               # the last ones bring score gradients out of float16's range
+        lens.copy_(torch.tensor([600 - 130 * i, 1 + 190 * i], dtype=torch.int32))
+        for gr, _ in graphs:
+            gr.replay()
+        M.gated_recurrence_gradient(dh[:, :300], x[:, :300], g[:, :300], x[:, :300])
+        torch.cuda.synchronize()
+        want = go()
+        for gr, res in graphs:
+            assert all(torch.equal(a, b) for a, b in zip(res, want)), i
+            assert not any(r.isnan().any() for r in res)
