@@ -65,8 +65,8 @@ int oph_seq_attn_gradient(const oph_seq_attn* a, int device, void* stream);
 
 /* ---- embedding ---------------------------------------------------------------------------------------------------------------
  * ids: n int32 or int64 (id_bytes 4 or 8).  lookup: out (n,units) contiguous = scale * table[id], table (vocab,units) of row stride
- * table_stride.  gradient: grad (vocab,units) contiguous = scale * sum of dout's rows whose id is the row, in ascending order of
- * the position, in float32; rows that no id names are 0.  zero_pad: id 0 reads as zeros and gets no gradient (modules.py:38-40).  An id outside
+ * table_stride.  gradient: grad (vocab,units) contiguous = scale * sum of dout's rows whose id is the row, in float32, in an
+ * order that only the call's sizes and dtype decide; rows that no id names are 0.  zero_pad: id 0 reads as zeros and gets no gradient (modules.py:38-40).  An id outside
  * 0..vocab-1 reads as zeros and adds to no row. */
 int oph_seq_embed_lookup(const void* ids, int id_bytes, int64_t n, const void* table, int64_t table_stride, int vocab, int units,
                          float scale, int zero_pad, int dtype, void* out, int device, void* stream);

@@ -351,9 +351,10 @@ static FwdPlan forward_plan(const oph_seq_attn* a) {
     f.wide = !f.few && cdiv(M, 128) * heads >= 256;
     f.rows = a->dtype == OPH_SEQ_F32 ? unit_rows<float>() : unit_rows<f16_t>();
     f.units = cdiv(M, f.rows) * heads;
-    // One round of workgroups (two a CU; fp32 with D > 128 holds one a CU): a second, partly filled one costs more than longer loops.  And
-    // at least 256 keys a split (fp32 128), since the join is a launch of its own: 16 x 200 rows over 150 keys x 64 bf16 take 7.0 us whole and
-    // 13.1 in two splits, 2 x 4 heads of 100 rows over 600 keys x 128 fp32 14.7 in four and 18.3 in two.
+    // 512 workgroups, 256 for fp32 with D > 128.  That is one round where a CU holds two (D <= 64) or, in the latter case, one; attn_split,
+    // attn16_forward and most of attn_few take more than half of a CU's registers above D = 64, and 512 are two rounds of those.  And at least
+    // 256 keys a split (fp32 128), since the join is a launch of its own: 16 x 200 rows over 150 keys x 64 bf16 take 7.0 us whole and 13.1 in two
+    // splits, 2 x 4 heads of 100 rows over 600 keys x 128 fp32 14.7 in four and 18.3 in two.
     const int64_t fill = (a->dtype == OPH_SEQ_F32 && a->D > 128 ? 256 : 512) / (f.units > 0 ? f.units : 1);
     const int64_t most = a->Tk / (a->dtype == OPH_SEQ_F32 && !f.few ? 128 : 256);
     const int64_t n = fill < most ? fill : most;

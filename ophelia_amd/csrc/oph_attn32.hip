@@ -2,7 +2,7 @@
 //
 // The fp32 matrix rate is a sixteenth of the 16-bit one, so operands come straight from memory (row pieces of 64 bytes, columns of 64 bytes)
 // and no tile of the other axis is shared through LDS.  What bounds them on long inputs is the return of these pieces (4 x 8 heads of 1024 x
-// 1024 x 256, gradient with respect to the queries: 675 us, 87 % of them busy with it, the matrix units half of the time); on short ones,
+// 1024 x 256, gradient with respect to the queries: 660 us, 87 % of them busy with it, the matrix units half of the time); on short ones,
 // which they are for, latency.  A workgroup owns 16 rows
 // (forward, dq) or 16 keys (dk, dv), whose operands its NW waves share in LDS; every wave takes every NW-th tile of 16 of the other axis, and
 // their results are added in a fixed order at the end.  16 instead of 32 rows halve both the work of a partly filled tile and the

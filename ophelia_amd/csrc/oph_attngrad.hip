@@ -392,7 +392,8 @@ static GradPlan gradient_plan(const oph_seq_attn* a) {
     const int rows = g.small ? 16 : 128, keys = g.small ? 16 : 128;
     g.dq_units = cdiv(M, rows) * heads;
     g.kv_units = cdiv(a->Tk, keys) * heads * (g.small || a->D <= 128 ? 1 : 2);
-    // one round of one or two workgroups a CU, at least 128 keys or rows a split (16 x 200 x 150 x 128 fp32: 36 us whole, 54 in two splits)
+    // 512 workgroups, 256 for D > 128: one round of two or one a CU; two rounds of attn16_dkv and of fp32 above D = 64, one of which fills a CU's
+    // registers.  At least 128 keys or rows a split (16 x 200 x 150 x 128 fp32: 36 us whole, 54 in two splits)
     const int64_t groups = a->D > 128 ? 256 : 512;
     g.dq_split = split_for(g.dq_units, a->Tk / 128, groups);
     g.kv_split = split_for(g.kv_units, M / 128, groups);

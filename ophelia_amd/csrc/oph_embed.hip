@@ -4,8 +4,8 @@
 // launch): each workgroup owns one bucket of rows (row mod buckets), reads all ids from the L2, keeps those of its bucket in LDS (or, where
 // one wave meets more than KEEP, reads them again) and learns from the same reading how many tokens lie in the buckets before its own.
 // embed_sum walks the sorted tokens in pieces, one run of equal rows after the other; a run inside a piece goes straight to the
-// gradient, what crosses a border is left in `part` and summed by embed_join in the order of the pieces.  No floating-point atomics: the
-// sums run in a fixed order.
+// gradient, what crosses a border is left in `part` and summed by embed_join, every fourth piece by one wave, then the four.  No floating-point
+// atomics: n, units and type alone decide the order of a sum.
 #include "oph_seq.h"
 #include "../../include/ophelia_hip.h"
 

@@ -18,7 +18,7 @@
 // bfloat16) that the forward's result is rounded by would be all that is left of the difference.  In float32 the result is the state and
 // is read; in 16 bits the states are formed again: a sequence of one block does so from the x and gate that it holds in registers, and for longer
 // ones a pass of the forward's chain leaves the state before every stretch in the workspace, from which the stretch is run once more.  4 x
-// 16384 x 1024 bf16: 129 us that pass, 225 the gradient; 120 and 288 with the states behind the blocks only, since composing the
+// 16384 x 1024 bf16: 126 us that pass, 208 the gradient; 120 and 288 with the states behind the blocks only, since composing the
 // stretches again takes 250 registers; 200 in one pass from the rounded states, which cost dgate up to all of its digits.
 #include "oph_seq.h"
 #include "../../include/ophelia_hip.h"
