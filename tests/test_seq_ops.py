@@ -224,3 +224,21 @@ def test_attention_refuses_what_one_launch_does_not_hold(lib, over):
         assert lib.oph_seq_attn_workspace(C.byref(a), 0) >= 0
     else:
         assert lib.oph_seq_attn_forward(C.byref(a), 0, None) == -4
+
+
+@pytest.mark.parametrize("dtype", [0, 1, 2])
+def test_recurrence_workspace_is_checked(lib, dtype):
+    """One block needs none; longer sequences do, and in 16 bits the gradient more than the forward."""
+    from ophelia_amd import _lib
+    a = _lib.OphSeqRecur()
+    for n in ("x", "gate", "h", "h_last", "dh", "dx", "dgate"):
+        setattr(a, n, 4096)
+    a.B, a.T, a.C, a.dtype = 2, 256, 40, dtype
+    assert lib.oph_seq_recur_workspace(C.byref(a), 0) == lib.oph_seq_recur_workspace(C.byref(a), 1) == 0
+    a.T = 257
+    need = [lib.oph_seq_recur_workspace(C.byref(a), g) for g in (0, 1)]
+    assert need[0] > 0 and (need[1] == need[0] if dtype == 0 else need[1] > 2 * need[0])
+    for g, call in enumerate((lib.oph_seq_recur_forward, lib.oph_seq_recur_gradient)):
+        for ws, size in ((None, need[g]), (4096, need[g] - 1), (4104, need[g])):
+            a.workspace, a.workspace_bytes = ws, size
+            assert call(C.byref(a), 0, None) == -1 and "workspace" in lib.oph_seq_last_error().decode()
